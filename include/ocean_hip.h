@@ -411,6 +411,65 @@ int och_gemm_split_plan(size_t M, size_t N, size_t K, unsigned tile_m, unsigned 
 int och_mgs_project(int dtype, size_t n, size_t k, const void *Q, ptrdiff_t ldq, void *v, void *r, och_stream stream);
 
 /* ======================================================================== */
+/* 8-bit floating point with block scales. No counterpart in the reference. */
+/* A matrix is held as 8-bit codes and a float scale per block of 128       */
+/* values (128 x 1, 1 x 128 or 128 x 128); code times scale is the value.   */
+/* All matrices are column-major with leading dimensions in elements, as    */
+/* och_gemm's: element (i, j) at i + j * ld. One token's features are a     */
+/* column. The scales of a matrix are a matrix of the same orientation: the */
+/* scale of element (i, j) at i / block_m + (j / block_n) * ldS.            */
+/* Three element types exist only here; they are no types of Ocean tensors. */
+/* Pointers are aligned to their element; sizes, leading dimensions and     */
+/* starts may be odd (whole 16-byte units are only faster). Matrices of one */
+/* call must not overlap unless stated. No call synchronises or allocates   */
+/* beyond the stream's workspace, so all can be recorded into a graph.      */
+/* ======================================================================== */
+enum { OCH_BFLOAT16 = 32, OCH_FLOAT8_E4M3 = 33, OCH_FLOAT8_E5M2 = 34 };     /* e4m3: largest value 448, no infinity; e5m2: 57344 */
+
+/* X (M x N; dtype half, bfloat16 or float) to codes Q (M x N bytes; `code` an 8-bit type) and scales S. block_m x block_n */
+/* is 128 x 1, 1 x 128 or 128 x 128; blocks at the border are shorter. For the largest magnitude m of a block and the     */
+/* largest code c:  a = max(m, 2^-100), S = a / c, Q = x * (c / a) rounded to nearest even (all in float). A block that   */
+/* holds an infinity or a NaN gets scale NaN and NaN codes, so that everything computed from it is NaN.                    */
+int och_quantize_blocks(int dtype, int code, size_t M, size_t N, const void *X, ptrdiff_t ldX, size_t block_m, size_t block_n,
+                        void *Q, ptrdiff_t ldQ, float *S, ptrdiff_t ldS, och_stream stream);
+
+/* Root-mean-square norm of every column ("row" of tokens) of the n x rows matrix X, in float:                             */
+/*    h = x + r rounded to dtype (h = x without R),  rstd = 1 / sqrt(mean(h^2) + eps),  y = (h * rstd) * w                 */
+/* dtype: half, bfloat16 or float, of X, R and H. R may be NULL; with R, H is required and receives the sum (it may be X   */
+/* or R itself, with the same leading dimension); without R, H may be NULL. W (n weights of type dtype_w: dtype or float)  */
+/* may be NULL (all 1). dtype_y: dtype, or an 8-bit type: Y then holds codes and S the scales of blocks of 128 x 1, made   */
+/* from y as och_quantize_blocks makes them, ready to be operand B of och_gemm_scaled. Without R, and with dtype_y equal   */
+/* to dtype, Y may be X itself. rstd (rows floats) may be NULL; the backward pass needs it. eps is at least 0.             */
+int och_rms_norm(int dtype, size_t n, size_t rows, const void *X, ptrdiff_t ldX, const void *R, ptrdiff_t ldR, void *H, ptrdiff_t ldH,
+                 int dtype_w, const void *W, float eps, int dtype_y, void *Y, ptrdiff_t ldY, float *S, ptrdiff_t ldS,
+                 float *rstd, och_stream stream);
+/* Its gradients. dY is the gradient of y (through the 8-bit rounding it passes unchanged), H what was normalised (X, or   */
+/* the sum that och_rms_norm stored), rstd as stored, dH the gradient that reaches h beside y (the residual stream's; may  */
+/* be NULL); all matrices of type dtype. With u = h * rstd and g = dy * w:                                                 */
+/*    dX = rstd * (g - u * mean(g * u)) + dh,   which is the gradient of x and of r;     dW = sum over the rows of dy * u  */
+/* dX may be dY or dH itself. dW (n floats, overwritten) may be NULL; it is summed in a fixed order that depends on the    */
+/* sizes alone, through the stream's workspace: n is at most 2^24 then.                                                    */
+int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *dY, ptrdiff_t lddY, const void *H, ptrdiff_t ldH, const float *rstd,
+                      int dtype_w, const void *W, const void *dH, ptrdiff_t lddH, void *dX, ptrdiff_t lddX, float *dW, och_stream stream);
+
+/* C <- alpha * sum_b SA(m, b) SB(b, n) sum_{k in block b} op(A)(m, k) op(B)(k, n) + beta * C, column-major: op(A) M x K,  */
+/* op(B) K x N, b = k / 128. dtypeA / dtypeB: 8-bit types, dtypeC: half, bfloat16 or float (one rounding, from float sums).*/
+/* transA, transB in {'N','T'} as in och_gemm. A scale of A covers blockA (1 or 128) rows of op(A) and 128 k; SA is the    */
+/* matrix of scales that och_quantize_blocks makes of the stored A with blocks of 128 x blockA ('T') or blockA x 128 ('N');*/
+/* B likewise: 128 x blockB ('N'), blockB x 128 ('T'). With the tokens' features as columns, weights W stored features-in  */
+/* x features-out and X features-in x tokens: the forward pass is 'T', 'N'; the input's gradient 'N', 'N' with A = W (its  */
+/* 128 x 128 scales serve both); the weights' gradient 'N', 'T' with A = X and B = dY quantized along the tokens.          */
+/* A float result has sums as good as float additions make them. For half and bfloat16 results the 8-bit matrix            */
+/* instruction adds eight products at a time and cuts off what lies below 2^-13 of the largest of them: about 1e-4 of the  */
+/* result's norm on Gaussian operands, less than the rounding to half.                                                     */
+/* beta = 0 does not read C; K = 0 leaves beta * C. Sums are added in an order that depends on sizes, leading dimensions   */
+/* and alignment alone: results are reproducible.                                                                          */
+int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, char transB, size_t M, size_t N, size_t K, float alpha,
+                    const void *A, ptrdiff_t ldA, const float *SA, ptrdiff_t ldSA, size_t blockA,
+                    const void *B, ptrdiff_t ldB, const float *SB, ptrdiff_t ldSB, size_t blockB,
+                    float beta, void *C, ptrdiff_t ldC, och_stream stream);
+
+/* ======================================================================== */
 /* Index operations (template_index.cu:37-57, index1.h:182, index2.h:188)   */
 /* ======================================================================== */
 int och_add_if_negative(int dtype, int ndims, const size_t *size, const ptrdiff_t *strides,

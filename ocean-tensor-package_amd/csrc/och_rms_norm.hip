@@ -1,0 +1,282 @@
+/* och_rms_norm and och_rms_norm_grad: the root-mean-square norm of the columns of a column-major n x rows matrix (one
+ * column per token, n features), with the residual stream's addition in front and, behind it, an output in the input's
+ * type or in 8-bit codes with one scale per 128 features; and its gradients. No counterpart in the reference.
+ *
+ *    h = round(x + r)          rstd = 1 / sqrt(mean(h^2) + eps)          y = (h rstd) w
+ *    g = dy w,  u = h rstd     dx = rstd (g - u mean(g u)) + dh          dw = sum over the rows of dy u
+ *
+ * The norm is that of the sum as it is stored, so that the backward pass, which reads the stored sum, differentiates the
+ * function that was computed. Sums are float. The gradient passes the 8-bit rounding straight through.
+ */
+#include "och_float8.h"
+
+namespace och {
+
+#define OCH_NORM_THREADS 256
+
+/* x of the lane that the DPP control names, added */
+template <int CTRL> __device__ __forceinline__ float dpp_add(float x)
+{  const int i = __float_as_int(x); return x + __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false)); }
+__device__ __forceinline__ float row16_sum(float x)
+{  x = dpp_add<0xB1>(x); x = dpp_add<0x4E>(x); x = dpp_add<0x141>(x); return dpp_add<0x140>(x); }
+__device__ __forceinline__ float lane_float(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+/* sum over the wave, in all lanes: a fixed tree */
+__device__ __forceinline__ float wave64_sum(float x)
+{  x = row16_sum(x);
+   return (lane_float(x, 0) + lane_float(x, 16)) + (lane_float(x, 32) + lane_float(x, 48));
+}
+/* sum over the workgroup, in all threads; `part` holds one float per wave and must not be in use */
+__device__ __forceinline__ float block_sum(float x, float *part)
+{  x = wave64_sum(x);
+   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+   __syncthreads();
+   float s = 0;
+   for (unsigned w = 0; w < blockDim.x / 64; w++) s += part[w];
+   __syncthreads();
+   return s;
+}
+
+struct NormParams
+{
+   const char *X, *R, *W; char *H, *Y; float *S, *rstd;
+   int64_t  ldX, ldR, ldH, ldY, ldS;    /* in elements */
+   int64_t  n, rows;
+   float    eps;
+   int      w_float;                    /* the weights are float (else the type of X) */
+};
+
+/* eight weights as floats (1 when there are none) */
+template <int DT> __device__ __forceinline__ void load_weights(const char *W, int w_float, int64_t at, int64_t valid, float *w)
+{  if (W == nullptr)
+   {
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = 1.0f;
+   }
+   else if (w_float)
+   {  Wide8<OCH_FLOAT> v; v.load(reinterpret_cast<const float *>(W) + at, valid);
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = v.get(e);
+   }
+   else
+   {  Wide8<DT> v; v.load(reinterpret_cast<const typename Wide<DT>::E *>(W) + at, valid);
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = v.get(e);
+   }
+}
+
+/* eight values of the output: rounded to the input's type, or to codes with a scale that sixteen lanes share.
+   Every lane of the wave calls it (CODE != 0 exchanges maxima between lanes). */
+template <int DT, int CODE> __device__ __forceinline__ void norm_store(const NormParams &p, int64_t row, int64_t at, int64_t valid, const float *y)
+{
+   if constexpr (CODE == 0)
+   {  Wide8<DT> o;
+#pragma unroll
+      for (int e = 0; e < 8; e++) o.put(e, y[e]);
+      o.store(reinterpret_cast<typename Wide<DT>::E *>(p.Y) + at + row * p.ldY, valid);
+   }
+   else
+   {  uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) m = umax(m, e < valid ? magnitude_bits(y[e]) : 0u);
+      float scale, factor; bool bad;
+      block_scale<CODE>(row16_max(m), scale, factor, bad);
+      och_u32x2 q;
+      q.x = code4<CODE>(y[0], y[1], y[2], y[3], factor, bad);
+      q.y = code4<CODE>(y[4], y[5], y[6], y[7], factor, bad);
+      store_codes(reinterpret_cast<uint8_t *>(p.Y) + at + row * p.ldY, q, valid);
+      if (at % OCH_F8_BLOCK == 0 && valid > 0) p.S[at / OCH_F8_BLOCK + row * p.ldS] = scale;
+   }
+}
+
+/* Rows of any length: a workgroup per row, two passes over it (the second finds it in the cache) */
+template <int DT, int CODE>
+__global__ __launch_bounds__(OCH_NORM_THREADS) void norm_long_kernel(const NormParams p)
+{
+   typedef typename Wide<DT>::E E;
+   __shared__ float part[OCH_NORM_THREADS / 64];
+   const int64_t row = blockIdx.x;
+   const E *x = reinterpret_cast<const E *>(p.X) + row * p.ldX, *r = reinterpret_cast<const E *>(p.R) + row * p.ldR;
+   E *h = reinterpret_cast<E *>(p.H) + row * p.ldH;
+   float sum = 0;
+   for (int64_t at = threadIdx.x * 8; at < p.n; at += OCH_NORM_THREADS * 8)
+   {  Wide8<DT> v;
+      v.load(x + at, p.n - at);
+      if (p.R)
+      {  Wide8<DT> a; a.load(r + at, p.n - at);
+#pragma unroll
+         for (int e = 0; e < 8; e++) v.put(e, v.get(e) + a.get(e));
+      }
+      if (p.H) v.store(h + at, p.n - at);
+      float s = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) s = __builtin_fmaf(v.get(e), v.get(e), s);
+      sum += s;
+   }
+   const float rstd = 1.0f / sqrtf(block_sum(sum, part) / (float)p.n + p.eps);
+   if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+   const E *again = p.H ? h : x;                           /* every thread reads what it wrote or read itself */
+   for (int64_t at0 = 0; at0 < p.n; at0 += OCH_NORM_THREADS * 8)
+   {  const int64_t at = at0 + threadIdx.x * 8;
+      Wide8<DT> v; float w[8], y[8];
+      v.load(again + at, p.n - at);
+      load_weights<DT>(p.W, p.w_float, at, p.n - at, w);
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = v.get(e) * rstd * w[e];
+      norm_store<DT, CODE>(p, row, at, p.n - at, y);
+   }
+}
+
+template <int DT, int CODE> static int norm_launch(const NormParams &p, hipStream_t stream)
+{
+   hipLaunchKernelGGL((norm_long_kernel<DT, CODE>), dim3((unsigned)p.rows), dim3(OCH_NORM_THREADS), 0, stream, p);
+   OCH_CHECK_LAUNCH();
+   return 0;
+}
+
+/* ---- gradients ------------------------------------------------------------------------------------------------------ */
+struct NormGradParams
+{
+   const char *dY, *H, *W, *dH; char *dX; const float *rstd; float *partial;   /* partial: n sums per workgroup, null when dW is not asked for */
+   int64_t  lddY, ldH, lddH, lddX;
+   int64_t  n, rows;
+   int      w_float;
+};
+
+/* Rows of any length: workgroup b takes rows b, b + G, ... and keeps its sums for dw in its own n floats of the workspace
+   (thread t always owns the same columns) */
+template <int DT>
+__global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_long_kernel(const NormGradParams p)
+{
+   typedef typename Wide<DT>::E E;
+   __shared__ float part[OCH_NORM_THREADS / 64];
+   float *mine = p.partial ? p.partial + (int64_t)blockIdx.x * p.n : nullptr;
+   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x)
+   {  const E *dy = reinterpret_cast<const E *>(p.dY) + row * p.lddY, *h = reinterpret_cast<const E *>(p.H) + row * p.ldH;
+      const float rstd = p.rstd[row];
+      float sum = 0;
+      for (int64_t at = threadIdx.x * 8; at < p.n; at += OCH_NORM_THREADS * 8)
+      {  Wide8<DT> a, b; float w[8], s = 0;
+         a.load(dy + at, p.n - at); b.load(h + at, p.n - at);
+         load_weights<DT>(p.W, p.w_float, at, p.n - at, w);
+#pragma unroll
+         for (int e = 0; e < 8; e++) s = __builtin_fmaf(a.get(e) * w[e], b.get(e) * rstd, s);
+         sum += s;
+      }
+      const float mean = block_sum(sum, part) / (float)p.n;
+      for (int64_t at = threadIdx.x * 8; at < p.n; at += OCH_NORM_THREADS * 8)
+      {  Wide8<DT> a, b, c, o; Wide8<OCH_FLOAT> d; float w[8];
+         const int64_t valid = p.n - at;
+         a.load(dy + at, valid); b.load(h + at, valid);
+         if (p.dH) c.load(reinterpret_cast<const E *>(p.dH) + row * p.lddH + at, valid);
+         load_weights<DT>(p.W, p.w_float, at, valid, w);
+         if (mine && row != blockIdx.x) d.load(mine + at, valid);
+         else
+         {
+#pragma unroll
+            for (int e = 0; e < 8; e++) d.put(e, 0.0f);
+         }
+#pragma unroll
+         for (int e = 0; e < 8; e++)
+         {  const float u = b.get(e) * rstd;
+            float x = rstd * (a.get(e) * w[e] - u * mean);
+            if (p.dH) x += c.get(e);
+            o.put(e, x);
+            d.put(e, __builtin_fmaf(a.get(e), u, d.get(e)));
+         }
+         o.store(reinterpret_cast<E *>(p.dX) + row * p.lddX + at, valid);
+         if (mine) d.store(mine + at, valid);
+      }
+   }
+}
+
+/* dw: the workgroups' sums, added in their order */
+__global__ __launch_bounds__(256) void norm_grad_finish_kernel(const float *partial, int64_t n, uint32_t groups, float *dW)
+{
+   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+   if (at >= n) return;
+   float s = 0;
+   for (uint32_t g = 0; g < groups; g++) s += partial[(int64_t)g * n + at];
+   dW[at] = s;
+}
+
+template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipStream_t stream)
+{
+   uint64_t groups = 2 * (uint64_t)gemm_compute_units();
+   if (groups > (uint64_t)p.rows) groups = (uint64_t)p.rows;
+   p.partial = nullptr;
+   if (dW)
+   {  const uint64_t fit = OCH_GEMM_WORKSPACE / ((uint64_t)p.n * sizeof(float));
+      char *ws;
+      if (fit == 0) return set_error("rms_norm_grad: rows of %lld features are too long for the weights' gradient", (long long)p.n);
+      if (groups > fit) groups = fit;
+      if (stream_gemm_workspace(stream, &ws) != 0) return -1;
+      p.partial = reinterpret_cast<float *>(ws);
+   }
+   hipLaunchKernelGGL((norm_grad_long_kernel<DT>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p);
+   OCH_CHECK_LAUNCH();
+   if (dW)
+   {  hipLaunchKernelGGL(norm_grad_finish_kernel, dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, stream, p.partial, p.n, (uint32_t)groups, dW);
+      OCH_CHECK_LAUNCH();
+   }
+   return 0;
+}
+
+static int check_weights(const char *name, int dtype, int dtype_w, const void *W)
+{
+   if (W == nullptr) return 0;
+   if (dtype_w != dtype && dtype_w != OCH_FLOAT) return set_error("%s: the weights are float or of the input's type (got %d)", name, dtype_w);
+   if ((uintptr_t)W % wide_size(dtype_w) != 0) return set_error("%s: misaligned pointer", name);
+   return 0;
+}
+
+} /* namespace och */
+
+using namespace och;
+
+extern "C" int och_rms_norm(int dtype, size_t n, size_t rows, const void *X, ptrdiff_t ldX, const void *R, ptrdiff_t ldR, void *H, ptrdiff_t ldH,
+                            int dtype_w, const void *W, float eps, int dtype_y, void *Y, ptrdiff_t ldY, float *S, ptrdiff_t ldS, float *rstd, och_stream stream)
+{
+   if (!wide_type(dtype)) return set_error("rms_norm is available for half, bfloat16 and float (got %d)", dtype);
+   if (dtype_y != dtype && !code_type(dtype_y)) return set_error("rms_norm: the output has the input's type, float8_e4m3 or float8_e5m2 (got %d)", dtype_y);
+   if (!(eps >= 0.0f)) return set_error("rms_norm: eps is negative or not a number");
+   const bool code = dtype_y != dtype;
+   if (n == 0 || rows == 0) return 0;
+   if (n > 0x7FFFFFFFull || rows > 0x7FFFFFFFull) return set_error("rms_norm: a side of %zu elements is too long", n > rows ? n : rows);
+   if (X == nullptr || Y == nullptr || (R != nullptr && H == nullptr) || (code && S == nullptr)) return set_error("rms_norm: null pointer argument");
+   const size_t blocks = (n + OCH_F8_BLOCK - 1) / OCH_F8_BLOCK;
+   if (ldX < (ptrdiff_t)n || ldY < (ptrdiff_t)n || (R && ldR < (ptrdiff_t)n) || (H && ldH < (ptrdiff_t)n) || (code && ldS < (ptrdiff_t)blocks))
+      return set_error("rms_norm: a leading dimension is smaller than the row (n = %zu)", n);
+   if (check_weights("rms_norm", dtype, dtype_w, W) != 0) return -1;
+   const size_t es = wide_size(dtype);
+   if ((uintptr_t)X % es || (uintptr_t)R % es || (uintptr_t)H % es || (!code && (uintptr_t)Y % es) || (uintptr_t)S % 4 || (uintptr_t)rstd % 4)
+      return set_error("rms_norm: misaligned pointer");
+   NormParams p;
+   p.X = (const char *)X; p.R = (const char *)R; p.W = (const char *)W; p.H = (char *)H; p.Y = (char *)Y; p.S = S; p.rstd = rstd;
+   p.ldX = ldX; p.ldR = ldR; p.ldH = ldH; p.ldY = ldY; p.ldS = ldS; p.n = (int64_t)n; p.rows = (int64_t)rows; p.eps = eps; p.w_float = (dtype_w == OCH_FLOAT);
+   hipStream_t s = as_stream(stream);
+#define OCH_GO(DT) (!code ? norm_launch<DT, 0>(p, s) : dtype_y == OCH_FLOAT8_E4M3 ? norm_launch<DT, OCH_FLOAT8_E4M3>(p, s) : norm_launch<DT, OCH_FLOAT8_E5M2>(p, s))
+   return OCH_BY_WIDE(dtype, OCH_GO);
+#undef OCH_GO
+}
+
+extern "C" int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *dY, ptrdiff_t lddY, const void *H, ptrdiff_t ldH, const float *rstd,
+                                 int dtype_w, const void *W, const void *dH, ptrdiff_t lddH, void *dX, ptrdiff_t lddX, float *dW, och_stream stream)
+{
+   if (!wide_type(dtype)) return set_error("rms_norm_grad is available for half, bfloat16 and float (got %d)", dtype);
+   if (n == 0) return 0;
+   if (n > 0x7FFFFFFFull || rows > 0x7FFFFFFFull) return set_error("rms_norm_grad: a side of %zu elements is too long", n > rows ? n : rows);
+   if (check_weights("rms_norm_grad", dtype, dtype_w, W) != 0) return -1;
+   if ((uintptr_t)dW % 4) return set_error("rms_norm_grad: misaligned pointer");
+   if (rows == 0) return dW ? fill_bytes(dW, 0, n * sizeof(float), as_stream(stream)) : 0;      /* a sum over nothing */
+   if (dY == nullptr || H == nullptr || rstd == nullptr || dX == nullptr) return set_error("rms_norm_grad: null pointer argument");
+   if (lddY < (ptrdiff_t)n || ldH < (ptrdiff_t)n || lddX < (ptrdiff_t)n || (dH && lddH < (ptrdiff_t)n))
+      return set_error("rms_norm_grad: a leading dimension is smaller than the row (n = %zu)", n);
+   const size_t es = wide_size(dtype);
+   if ((uintptr_t)dY % es || (uintptr_t)H % es || (uintptr_t)dH % es || (uintptr_t)dX % es || (uintptr_t)rstd % 4) return set_error("rms_norm_grad: misaligned pointer");
+   NormGradParams p;
+   p.dY = (const char *)dY; p.H = (const char *)H; p.W = (const char *)W; p.dH = (const char *)dH; p.dX = (char *)dX; p.rstd = rstd; p.partial = nullptr;
+   p.lddY = lddY; p.ldH = ldH; p.lddH = lddH; p.lddX = lddX; p.n = (int64_t)n; p.rows = (int64_t)rows; p.w_float = (dtype_w == OCH_FLOAT);
+#define OCH_GO(DT) norm_grad_launch<DT>(p, dW, as_stream(stream))
+   return OCH_BY_WIDE(dtype, OCH_GO);
+#undef OCH_GO
+}

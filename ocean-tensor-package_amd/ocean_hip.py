@@ -19,6 +19,8 @@ MAX_DIMS = 8
  HALF, FLOAT, DOUBLE, CHALF, CFLOAT, CDOUBLE) = range(15)
 DTYPE_NAMES = ["bool", "uint8", "uint16", "uint32", "uint64", "int8", "int16", "int32", "int64",
                "half", "float", "double", "chalf", "cfloat", "cdouble"]
+# element types of the block-scaled 8-bit operations alone; no types of Ocean tensors
+BFLOAT16, FLOAT8_E4M3, FLOAT8_E5M2 = 32, 33, 34
 TYPE_SIZE = [1, 1, 2, 4, 8, 1, 2, 4, 8, 2, 4, 8, 4, 8, 16]
 # numpy storage dtype per element type; half travels as its 16-bit pattern, chalf as two of them
 NP_STORAGE = [np.uint8, np.uint8, np.uint16, np.uint32, np.uint64, np.int8, np.int16, np.int32, np.int64,
@@ -204,6 +206,12 @@ PROTOTYPES = {
     "och_gemm_batched": (_i, [_i, C.c_char, C.c_char, C.c_size_t, C.c_size_t, C.c_size_t, _vp, _vp, C.c_ssize_t, _vp, C.c_ssize_t,
                               _vp, _vp, C.c_ssize_t, _i, _sz, _st, _st, _st, _st, _st, _i, _vp]),
     "och_mgs_project": (_i, [_i, C.c_size_t, C.c_size_t, _vp, C.c_ssize_t, _vp, _vp, _vp]),
+    "och_quantize_blocks": (_i, [_i, _i, C.c_size_t, C.c_size_t, _vp, C.c_ssize_t, C.c_size_t, C.c_size_t, _vp, C.c_ssize_t, _vp, C.c_ssize_t, _vp]),
+    "och_rms_norm": (_i, [_i, C.c_size_t, C.c_size_t, _vp, C.c_ssize_t, _vp, C.c_ssize_t, _vp, C.c_ssize_t, _i, _vp, C.c_float, _i, _vp, C.c_ssize_t,
+                          _vp, C.c_ssize_t, _vp, _vp]),
+    "och_rms_norm_grad": (_i, [_i, C.c_size_t, C.c_size_t, _vp, C.c_ssize_t, _vp, C.c_ssize_t, _vp, _i, _vp, _vp, C.c_ssize_t, _vp, C.c_ssize_t, _vp, _vp]),
+    "och_gemm_scaled": (_i, [_i, _i, _i, C.c_char, C.c_char, C.c_size_t, C.c_size_t, C.c_size_t, C.c_float, _vp, C.c_ssize_t, _vp, C.c_ssize_t, C.c_size_t,
+                             _vp, C.c_ssize_t, _vp, C.c_ssize_t, C.c_size_t, C.c_float, _vp, C.c_ssize_t, _vp]),
     "och_add_if_negative": (_i, [_i, _i, _sz, _st, _vp, Scalar, _vp]),
     "och_index_to_offset": (_i, [_i, _i, C.POINTER(C.c_int64), C.c_ssize_t, C.c_size_t, C.c_ssize_t, _vp, C.c_ssize_t, _vp, _vp]),
     "och_get_index": (_i, [_i, _i, _sz, C.POINTER(C.POINTER(C.c_int64)), _st, _vp, _st, _vp, _vp]),
