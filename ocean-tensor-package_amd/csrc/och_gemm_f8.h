@@ -22,7 +22,15 @@ struct F8GemmParams
    float    alpha, beta;
    int      dtypeC;
    uint32_t tiles_m, tiles_n;
+   /* few tiles and a long K: workgroup (x, y) computes share y of tile x, share_slabs blocks of 128 k, and leaves its sums
+      in plane y of `partial`; a second kernel adds the planes in order. 0: every tile has the whole K */
+   uint32_t share_slabs;
+   float   *partial;
 };
+int gemm_f8_tile_44(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_45(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_54(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_55(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
 
 typedef __bf16 och_bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 och_bf16x8 __attribute__((ext_vector_type(8)));

@@ -38,8 +38,8 @@ template <bool KC, int R> struct F8Slab
       multiple of 8): in every group of 16 lanes, lanes 2 e and 2 e + 1 read the 16 rows of k0 + e, and lane i of the group
       receives row i of k0 .. k0 + 7 */
    static OCH_SLAB_FN uint32_t at_k(uint32_t row0, uint32_t k0, uint32_t lane)
-   {  const uint32_t k = k0 + (lane % 16) / 2;
-      return k * R + 16 * ((row0 / 16) ^ twist(k)) + 8 * (lane % 2);
+   {  const uint32_t e = (lane % 16) / 2;              /* twist(k0 + e) is twist(e) */
+      return (k0 + e) * R + 16 * ((row0 / 16) ^ twist(e)) + 8 * (lane % 2);
    }
 };
 

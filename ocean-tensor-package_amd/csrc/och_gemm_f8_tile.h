@@ -1,0 +1,291 @@
+/* The block-scaled product on tiles of 128 x 128 for any operands: whatever their alignment, sizes and scales.
+ *
+ * Four waves own 64 x 64 of the tile each. A slab of 128 k of both operands and the slab's scales pass through registers
+ * to one of two LDS buffers: the loads of slab s + 1 are issued before the matrix instructions of slab s and stored behind
+ * them, one barrier per slab, two workgroups per compute unit. Chunks of 16 bytes are single loads whatever their
+ * alignment; at the matrix's border they are loaded byte by byte.
+ *
+ * ROWS: the scale of A differs between the rows of a wave (blockA = 1): a multiplication more per element and slab. */
+#pragma once
+#include "och_gemm_f8.h"
+
+namespace och {
+
+#define OCH_F8_TILE 128
+#define OCH_F8_TILE_THREADS 256
+
+/* Order of the tiles: workgroups go to the eight compute dies in turn, each with a cache of its own, so every die gets a
+   contiguous run of tiles; inside the run tiles advance in strips of eight rows of tiles, so that the tiles of a die that
+   are in flight together share operands */
+__device__ __forceinline__ void f8_tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm, uint32_t &tn)
+{
+   const uint32_t total = tiles_m * tiles_n, q = total / 8, r = total % 8, die = id % 8;
+   id = die * q + (die < r ? die : r) + id / 8;
+   const uint32_t strip = id / (8 * tiles_n), first = strip * 8, height = tiles_m - first < 8 ? tiles_m - first : 8, in = id - first * tiles_n;
+   tm = first + in % height; tn = in / height;
+}
+
+/* 16 bytes moved towards their start by `by` bytes (16 or more: zero), zeros behind */
+static __device__ __forceinline__ och_u32x4 f8_shift(och_u32x4 v, uint32_t by)
+{  uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+   const uint32_t bits = 8 * (by & 7);
+   if (by & 8) { lo = hi; hi = 0; }
+   lo = bits ? (lo >> bits | hi << (64 - bits)) : lo;
+   hi >>= bits;
+   if (by >= 16) lo = hi = 0;
+   v.x = (uint32_t)lo; v.y = (uint32_t)(lo >> 32); v.z = (uint32_t)hi; v.w = (uint32_t)(hi >> 32);
+   return v;
+}
+/* a chunk of which the first `valid` bytes exist (none when valid <= 0), the others zero; `length`: bytes of the run of
+   memory that it ends (from 16 on, the 16 bytes up to its end are one load) */
+static __device__ __forceinline__ och_u32x4 f8_border_chunk(const uint8_t *at, int64_t valid, uint32_t length)
+{
+   och_u32x4 v = { 0, 0, 0, 0 };
+   if (valid >= 16) v = *reinterpret_cast<const och_u32x4_any *>(at);
+   else if (valid > 0 && length >= 16) v = f8_shift(*reinterpret_cast<const och_u32x4_any *>(at + valid - 16), (uint32_t)(16 - valid));
+   else if (valid > 0)
+   {  uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+      for (int e = 0; e < valid; e++)
+      {  const uint64_t b = at[e];
+         if (e < 8) lo |= b << (8 * e); else hi |= b << (8 * (e - 8));
+      }
+      v.x = (uint32_t)lo; v.y = (uint32_t)(lo >> 32); v.z = (uint32_t)hi; v.w = (uint32_t)(hi >> 32);
+   }
+   return v;
+}
+
+/* The chunks that a thread moves: threadIdx.x + THREADS i of every slab. They differ by whole rows (KC) or whole k (!KC)
+   with the same twist. Rows that do not exist are never loaded: KC repeats the last row instead; !KC loads the last 16
+   rows where a chunk passes the end, and moves them into place on the way to LDS (so `rows` is at least 16 there). What
+   these lanes hold for rows outside the matrix reaches only elements of C that are not written. */
+template <bool KC, int R, int THREADS> struct F8Stage
+{
+   typedef F8Slab<KC, R> L;
+   static constexpr int NV = (int)L::CHUNKS / THREADS, NP = KC ? NV : 1;
+   static constexpr uint32_t STEP = KC ? THREADS / 8 : THREADS / L::PER_K;       /* rows or k from a thread's chunk to its next */
+   static_assert(STEP % 8 == 0, "the twist must not change from chunk to chunk");
+   och_u32x4 v[NV];
+   const uint8_t *at[NP];
+   uint32_t move;
+   static __device__ __forceinline__ bool pipelined(uint32_t rows) { return KC || rows >= 16; }
+   __device__ __forceinline__ void start(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows)
+   {  uint32_t row, k;
+      L::where(threadIdx.x, row, k);
+      if (KC)
+      {
+#pragma unroll
+         for (int i = 0; i < NP; i++)
+         {  const uint32_t r = r0 + row + i * STEP;
+            at[i] = mat + (int64_t)(k0 + k) + (int64_t)(r < rows ? r : rows - 1) * ld;
+         }
+         move = 0;
+      }
+      else
+      {  const uint32_t r = r0 + row, last = rows >= 16 ? rows - 16 : 0, from = r < last ? r : last;
+         at[0] = mat + from + (int64_t)(k0 + k) * ld;
+         move = r - from;
+      }
+   }
+   /* the next slab, whole along k */
+   __device__ __forceinline__ void load(int64_t ld)
+   {
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+      {  v[i] = *reinterpret_cast<const och_u32x4_any *>(KC ? at[i % NP] : at[0] + i * (int64_t)STEP * ld);
+         if (KC) at[i % NP] += OCH_F8_SLAB;
+      }
+      if (!KC) at[0] += OCH_F8_SLAB * ld;
+   }
+   /* any slab, chunk by chunk */
+   __device__ __forceinline__ void load_border(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows, uint32_t K)
+   {  move = 0;
+      uint32_t thread = threadIdx.x;
+      asm volatile("" : "+v"(thread));   /* what follows from it is computed here, not kept in registers through the pipelined slabs */
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+      {  uint32_t row, k;
+         L::where(thread + THREADS * i, row, k);
+         const int64_t gr = (int64_t)r0 + row, gk = (int64_t)k0 + k;
+         const int64_t valid = KC ? (gr < rows ? (int64_t)K - gk : 0) : (gk < K ? (int64_t)rows - gr : 0);
+         v[i] = f8_border_chunk(mat + (KC ? gk + gr * ld : gr + gk * ld), valid, KC ? K : rows);
+      }
+   }
+   __device__ __forceinline__ void store(char *slab, bool border)
+   {
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+      {  if (!KC && border) v[i] = f8_shift(v[i], move);
+         *reinterpret_cast<och_u32x4 *>(slab + 16 * (threadIdx.x + THREADS * i)) = v[i];
+      }
+   }
+};
+
+/* four neighbouring rows of one column of C */
+template <int DT> __device__ __forceinline__ void f8_finish4(char *C, int64_t at, och_f32x4v s, float alpha, float beta, uint32_t valid)
+{
+   typedef typename Wide<DT>::E E;
+   typedef E E4 __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+   E *c = reinterpret_cast<E *>(C) + at;
+   if (valid >= 4)
+   {  E4 o;
+      if (beta != 0.0f)
+      {  const E4 old = *reinterpret_cast<const E4 *>(c);
+#pragma unroll
+         for (int r = 0; r < 4; r++) o[r] = Wide<DT>::put(__builtin_fmaf(beta, Wide<DT>::get(old[r]), alpha * s[r]));
+      }
+      else
+      {
+#pragma unroll
+         for (int r = 0; r < 4; r++) o[r] = Wide<DT>::put(alpha * s[r]);
+      }
+      *reinterpret_cast<E4 *>(c) = o;
+   }
+   else
+   {
+#pragma unroll
+      for (int r = 0; r < 3; r++) if ((uint32_t)r < valid) f8_finish<DT>(C, at + r, s[r], alpha, beta);
+   }
+}
+/* A wave's TI x TJ tiles of 16 x 16 to C: lane l holds rows 4 (l / 16) .. + 3 of column l mod 16 of every tile; m, n: this
+   lane's place in the first. One tile after the other (the fences), or the compiler keeps all addresses at once. */
+template <int DT, int TI, int TJ> __device__ __forceinline__ void f8_write(const F8GemmParams &p, uint32_t m, uint32_t n, const och_f32x4v (&acc)[TI][TJ])
+{
+#pragma unroll
+   for (int j = 0; j < TJ; j++)
+   {  if (n + 16 * j < p.N)
+      {  const int64_t column = (int64_t)(n + 16 * j) * p.ldC;
+#pragma unroll
+         for (int i = 0; i < TI; i++)
+            if (m + 16 * i < p.M) f8_finish4<DT>(p.C, column + m + 16 * i, acc[i][j], p.alpha, p.beta, p.M - m - 16 * i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+   }
+}
+/* ... or, for a share of K, as raw sums into the share's plane (M x N, dense) */
+template <int TI, int TJ> __device__ __forceinline__ void f8_write_share(const F8GemmParams &p, uint32_t share, uint32_t m, uint32_t n, const och_f32x4v (&acc)[TI][TJ])
+{
+   F8GemmParams q = p;
+   q.C = reinterpret_cast<char *>(p.partial + (size_t)share * p.M * p.N); q.ldC = p.M; q.alpha = 1.0f; q.beta = 0.0f;
+   f8_write<OCH_FLOAT, TI, TJ>(q, m, n, acc);
+}
+template <int TI, int TJ> __device__ __forceinline__ void f8_write_any(const F8GemmParams &p, uint32_t share, uint32_t m, uint32_t n, const och_f32x4v (&acc)[TI][TJ])
+{
+   if (p.share_slabs)              f8_write_share<TI, TJ>(p, share, m, n, acc);
+   else if (p.dtypeC == OCH_FLOAT) f8_write<OCH_FLOAT, TI, TJ>(p, m, n, acc);
+   else if (p.dtypeC == OCH_HALF)  f8_write<OCH_HALF, TI, TJ>(p, m, n, acc);
+   else                            f8_write<OCH_BFLOAT16, TI, TJ>(p, m, n, acc);
+}
+
+template <bool AKC, bool BKC, bool E5A, bool E5B, bool WIDE, bool ROWS>
+__global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(const F8GemmParams p)
+{
+   constexpr int R = OCH_F8_TILE, THREADS = OCH_F8_TILE_THREADS, OPERAND = R * OCH_F8_SLAB, BUF = 2 * OPERAND + 2 * R * 4;
+   __shared__ __align__(16) char lds[2 * BUF];
+   uint32_t tm, tn;
+   f8_tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+   const uint32_t m0 = tm * R, n0 = tn * R;
+   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % 2 * 64, wn = wave / 2 * 64;
+   const och_f32x4v zero = { 0, 0, 0, 0 };
+   och_f32x4v acc[4][4];
+#pragma unroll
+   for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[i][j] = zero;
+
+   const uint32_t all = (p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB;
+   uint32_t s = 0, end = all;
+   if (p.share_slabs) { s = blockIdx.y * p.share_slabs; end = s + p.share_slabs < all ? s + p.share_slabs : all; }
+
+   /* every thread brings one scale: threads 0 .. 127 of A's rows, 128 .. 255 of B's columns; those outside C repeat the last */
+   const bool forA = threadIdx.x < R;
+   const uint32_t line = forA ? m0 + threadIdx.x : n0 + threadIdx.x - R, most = (forA ? p.M : p.N) - 1;
+   const float *scale = forA ? p.SA + (int64_t)((line < most ? line : most) >> p.shiftA) * p.sa_m : p.SB + (int64_t)((line < most ? line : most) >> p.shiftB) * p.sb_n;
+   const int64_t scale_step = forA ? p.sa_k : p.sb_k;
+
+   /* slabs that are whole along k are pipelined; the rest of K, and everything of an operand of under 16 contiguous rows, is not */
+   const uint32_t whole = p.K / OCH_F8_SLAB, piped = !F8Stage<AKC, R, THREADS>::pipelined(p.M) || !F8Stage<BKC, R, THREADS>::pipelined(p.N) ? s : end < whole ? end : whole;
+   const bool borderA = m0 + R > p.M, borderB = n0 + R > p.N;
+   F8Stage<AKC, R, THREADS> la; F8Stage<BKC, R, THREADS> lb; float ls = 0;
+   la.start(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M); lb.start(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N);
+   auto stash = [&](char *buf)
+   {  la.store(buf, borderA); lb.store(buf + OPERAND, borderB);
+      reinterpret_cast<float *>(buf + 2 * OPERAND)[threadIdx.x] = ls;
+   };
+   if (s < piped)
+   {  la.load(p.ldA); lb.load(p.ldB); ls = scale[(int64_t)s * scale_step];
+      stash(lds);
+   }
+   __syncthreads();
+   for (uint32_t turn = 0; s < end; s++, turn ^= 1)
+   {  char *buf = lds + turn * BUF;
+      const float *sA = reinterpret_cast<const float *>(buf + 2 * OPERAND), *sB = sA + R;
+      if (s >= piped)
+      {  la.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); lb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); ls = scale[(int64_t)s * scale_step];
+         stash(buf);
+         __syncthreads();
+      }
+      const bool more = s + 1 < piped;
+      if (more) { la.load(p.ldA); lb.load(p.ldB); ls = scale[(int64_t)(s + 1) * scale_step]; }
+      F8Operand<WIDE> b[4]; float t[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+      {  b[j].template set<E5B>(f8_fragment<BKC, R>(buf + OPERAND, wn + 16 * j));
+         t[j] = sB[wn + 16 * j + lane % 16];
+         if (!ROWS) t[j] *= sA[wm];
+         __builtin_amdgcn_sched_barrier(0);
+      }
+      /* step i: the fragment of row i + 1 is read, row i multiplied, the sums of row i - 1 scaled and added; the fences keep
+         the compiler from collecting more rows' sums than registers hold */
+      och_i32x8 codes = f8_fragment<AKC, R>(buf, wm);
+      och_f32x4v part[2][4], rs[2];
+#pragma unroll
+      for (int i = 0; i <= 4; i++)
+      {  if (i < 4)
+         {  F8Operand<WIDE> a;
+            a.template set<E5A>(codes);
+            if (i < 3) codes = f8_fragment<AKC, R>(buf, wm + 16 * (i + 1));
+            if (ROWS) rs[i % 2] = *reinterpret_cast<const och_f32x4v *>(sA + wm + 16 * i + 4 * (lane / 16));
+#pragma unroll
+            for (int j = 0; j < 4; j++) part[i % 2][j] = f8_block<E5A, E5B>(a, b[j]);
+         }
+         if (i > 0)
+         {  const int o = (i - 1) % 2;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+               for (int r = 0; r < 4; r++) acc[i > 0 ? i - 1 : 0][j][r] = __builtin_fmaf(part[o][j][r], ROWS ? rs[o][r] * t[j] : t[j], acc[i > 0 ? i - 1 : 0][j][r]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) asm volatile("" : "+v"(acc[i > 0 ? i - 1 : 0][j]));      /* here, not behind the loop's last branch */
+         }
+         if (i > 0 && i < 4)
+         {  /* one block's matrix instructions, then the additions of a block of the row before */
+#pragma unroll
+            for (int j = 0; j < 4; j++) { __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0); __builtin_amdgcn_sched_group_barrier(0x2, ROWS ? 8 : 4, 0); }
+         }
+         __builtin_amdgcn_sched_barrier(0);
+      }
+      if (more) stash(lds + (turn ^ 1) * BUF);
+      __syncthreads();
+   }
+   f8_write_any<4, 4>(p, blockIdx.y, m0 + wm + 4 * (lane / 16), n0 + wn + lane % 16, acc);
+}
+
+template <bool E5A, bool E5B, bool WIDE, bool ROWS> static int gemm_f8_tile_launch(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream)
+{
+   const dim3 block(OCH_F8_TILE_THREADS);
+   if (akc && bkc) hipLaunchKernelGGL((gemm_f8_tile_kernel<true, true, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
+   else if (akc)   hipLaunchKernelGGL((gemm_f8_tile_kernel<true, false, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
+   else if (bkc)   hipLaunchKernelGGL((gemm_f8_tile_kernel<false, true, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
+   else            hipLaunchKernelGGL((gemm_f8_tile_kernel<false, false, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
+   OCH_CHECK_LAUNCH();
+   return 0;
+}
+template <bool E5A, bool E5B> static int gemm_f8_tile(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream)
+{
+   const bool wide = p.dtypeC == OCH_FLOAT, rows = p.shiftA == 0;
+   return wide ? (rows ? gemm_f8_tile_launch<E5A, E5B, true, true>(p, akc, bkc, grid, stream) : gemm_f8_tile_launch<E5A, E5B, true, false>(p, akc, bkc, grid, stream))
+               : (rows ? gemm_f8_tile_launch<E5A, E5B, false, true>(p, akc, bkc, grid, stream) : gemm_f8_tile_launch<E5A, E5B, false, false>(p, akc, bkc, grid, stream));
+}
+
+} /* namespace och */
