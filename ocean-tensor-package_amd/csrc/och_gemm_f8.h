@@ -31,6 +31,10 @@ int gemm_f8_tile_44(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStr
 int gemm_f8_tile_45(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
 int gemm_f8_tile_54(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
 int gemm_f8_tile_55(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
+int gemm_f8_few_44(const F8GemmParams &p, hipStream_t stream);
+int gemm_f8_few_45(const F8GemmParams &p, hipStream_t stream);
+int gemm_f8_few_54(const F8GemmParams &p, hipStream_t stream);
+int gemm_f8_few_55(const F8GemmParams &p, hipStream_t stream);
 
 typedef __bf16 och_bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 och_bf16x8 __attribute__((ext_vector_type(8)));

@@ -86,5 +86,9 @@ extern "C" int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, 
    p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K; p.alpha = alpha; p.beta = beta; p.dtypeC = dtypeC;
    const bool e5a = dtypeA == OCH_FLOAT8_E5M2, e5b = dtypeB == OCH_FLOAT8_E5M2;
    hipStream_t s = as_stream(stream);
+   /* few columns on their own kernel, which loads 16 bytes at a time and counts bytes within its rows in 32 bits */
+   const bool aligned = (((uintptr_t)A | (uintptr_t)B | (uintptr_t)ldA | (uintptr_t)ldB) & 15) == 0, near = ldA < (1 << 25) && ldB < (1 << 25);
+   if (N <= 64 && akc && bkc && aligned && near)
+      return e5a ? (e5b ? gemm_f8_few_55(p, s) : gemm_f8_few_54(p, s)) : (e5b ? gemm_f8_few_45(p, s) : gemm_f8_few_44(p, s));
    return gemm_f8_tiles(p, e5a, e5b, akc, bkc, s);
 }

@@ -479,3 +479,18 @@ def test_gemm_is_reproducible(hip, stream):
         first = run_gemm(stream, F.E4M3, F.E4M3, F.FLOAT, "T", "N", a, sa, 128, b, sb, 1)
         for _ in range(3):
             assert np.array_equal(first.view(np.uint32), run_gemm(stream, F.E4M3, F.E4M3, F.FLOAT, "T", "N", a, sa, 128, b, sb, 1).view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype", [F.FLOAT, F.HALF], ids=name_of)
+@pytest.mark.parametrize("ba,bb", [(128, 1), (1, 1), (128, 128)])
+def test_gemm_few_columns(hip, stream, dtype, ba, bb):
+    """One to a few columns, bit for bit: every number of tiles of 16 columns, K from one code to many slabs with ends of all
+    lengths, M that leaves rows of the last tile empty, odd leading dimensions."""
+    rng = np.random.default_rng(dtype + ba + bb)
+    for k, (M, N, K) in enumerate([(1, 1, 1), (17, 1, 5), (16, 2, 15), (40, 3, 17), (128, 1, 127), (130, 5, 129), (96, 15, 255), (64, 16, 1000), (200, 17, 1025),
+                                   (48, 31, 2047), (33, 33, 640), (256, 48, 4096), (100, 63, 3333), (1040, 64, 384), (4100, 1, 4112), (5000, 40, 208)]):
+        a, sa, b, sb = exact_case(rng, M, N, K, ba, bb)
+        pad = [0, 16, 3][k % 3]
+        got = run_gemm(stream, F.E4M3, F.E4M3, dtype, "T", "N", a, sa, ba, b, sb, bb, pad=(pad, pad, pad), shift=(pad, 2 * pad, pad), spad=k % 2)
+        av, bv = F.decode(a, F.E4M3) * wide_scales(sa, ba, M, K), F.decode(b, F.E4M3) * wide_scales(sb, bb, N, K)
+        assert np.array_equal(got, F.to_wide(bv.astype(np.float32) @ av.astype(np.float32).T, dtype)), (M, N, K)
