@@ -31,6 +31,10 @@ int gemm_f8_tile_44(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStr
 int gemm_f8_tile_45(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
 int gemm_f8_tile_54(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
 int gemm_f8_tile_55(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
+int gemm_f8_pipe_44(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);
+int gemm_f8_pipe_45(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);
+int gemm_f8_pipe_54(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);
+int gemm_f8_pipe_55(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);
 int gemm_f8_few_44(const F8GemmParams &p, hipStream_t stream);
 int gemm_f8_few_45(const F8GemmParams &p, hipStream_t stream);
 int gemm_f8_few_54(const F8GemmParams &p, hipStream_t stream);

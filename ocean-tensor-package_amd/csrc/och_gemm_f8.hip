@@ -6,6 +6,7 @@
  * outside them, four multiply-adds per lane beside 32 or 64 cycles of matrix work.
  */
 #include "och_gemm_f8_tile.h"
+#include <math.h>
 
 namespace och {
 
@@ -51,6 +52,15 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
    return 0;
 }
 
+/* Whether a product of aligned operands is quicker on 256 x 256 tiles (one workgroup per compute unit) than on 128 x 128
+   (two): rounds of the compute units times the work of a round over its rate. Measured rates on full rounds: 2.3 and 1.5
+   PFLOP/s. */
+static bool gemm_f8_large(size_t M, size_t N)
+{
+   const double units = gemm_compute_units(), small = (double)((M + 127) / 128) * (double)((N + 127) / 128), large = (double)((M + 255) / 256) * (double)((N + 255) / 256);
+   return ceil(large / units) * 4 / 2.3 < ceil(small / (2 * units)) * 2 / 1.5;
+}
+
 } /* namespace och */
 
 using namespace och;
@@ -90,5 +100,11 @@ extern "C" int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, 
    const bool aligned = (((uintptr_t)A | (uintptr_t)B | (uintptr_t)ldA | (uintptr_t)ldB) & 15) == 0, near = ldA < (1 << 25) && ldB < (1 << 25);
    if (N <= 64 && akc && bkc && aligned && near)
       return e5a ? (e5b ? gemm_f8_few_55(p, s) : gemm_f8_few_54(p, s)) : (e5b ? gemm_f8_few_45(p, s) : gemm_f8_few_44(p, s));
+   /* float results need the wide sums, and chunks of 16 rows must not pass the end of an operand that is contiguous along them */
+   if (dtypeC != OCH_FLOAT && aligned && ldA < (1 << 24) && ldB < (1 << 24) && ldSA < (1 << 22) && ldSB < (1 << 22) && (akc || M % 16 == 0) && (bkc || N % 16 == 0) && gemm_f8_large(M, N))
+   {  p.tiles_m = (p.M + 255) / 256; p.tiles_n = (p.N + 255) / 256;
+      if ((uint64_t)p.tiles_m * p.tiles_n > 0x7FFFFFFFull) return set_error("gemm_scaled: too many tiles");
+      return e5a ? (e5b ? gemm_f8_pipe_55(p, akc, bkc, s) : gemm_f8_pipe_54(p, akc, bkc, s)) : (e5b ? gemm_f8_pipe_45(p, akc, bkc, s) : gemm_f8_pipe_44(p, akc, bkc, s));
+   }
    return gemm_f8_tiles(p, e5a, e5b, akc, bkc, s);
 }

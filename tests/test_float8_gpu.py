@@ -494,3 +494,18 @@ def test_gemm_few_columns(hip, stream, dtype, ba, bb):
         got = run_gemm(stream, F.E4M3, F.E4M3, dtype, "T", "N", a, sa, ba, b, sb, bb, pad=(pad, pad, pad), shift=(pad, 2 * pad, pad), spad=k % 2)
         av, bv = F.decode(a, F.E4M3) * wide_scales(sa, ba, M, K), F.decode(b, F.E4M3) * wide_scales(sb, bb, N, K)
         assert np.array_equal(got, F.to_wide(bv.astype(np.float32) @ av.astype(np.float32).T, dtype)), (M, N, K)
+
+
+@pytest.mark.parametrize("ba,bb", [(128, 1), (1, 1)])
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_gemm_large(hip, stream, ta, tb, ba, bb):
+    """Products of several hundred large tiles, whole and ragged, bit for bit against the product of the exact values by
+    probes: C x for a vector of small whole numbers (every number below 2^53), and a few columns in full."""
+    rng = np.random.default_rng(ba + ord(tb))
+    for M, N, K in [(4096, 4096, 256), (4096 + 16, 3840 + 272, 400), (3856, 4352, 144)]:
+        a, sa, b, sb = exact_case(rng, M, N, K, ba, bb)
+        got = F.from_wide(run_gemm(stream, F.E4M3, F.E4M3, F.BF16, ta, tb, a, sa, ba, b, sb, bb), F.BF16)
+        av = (F.decode(a, F.E4M3) * wide_scales(sa, ba, M, K)).astype(np.float32)
+        bv = (F.decode(b, F.E4M3) * wide_scales(sb, bb, N, K)).astype(np.float32)
+        want = F.from_wide(F.to_wide(bv @ av.T, F.BF16), F.BF16)        # whole multiples of 1/4 below 2^22: exact in float
+        assert np.array_equal(got, want), (M, N, K, np.argwhere(got != want)[:5])
