@@ -55,6 +55,15 @@ static __device__ __forceinline__ och_u32x4 f8_border_chunk(const uint8_t *at, i
    return v;
 }
 
+/* chunk q of a slab, wherever it lies with respect to the matrix's ends */
+template <bool KC, int R> static __device__ __forceinline__ och_u32x4 f8_any_chunk(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows, uint32_t K, uint32_t q)
+{  uint32_t row, k;
+   F8Slab<KC, R>::where(q, row, k);
+   const int64_t gr = (int64_t)r0 + row, gk = (int64_t)k0 + k;
+   const int64_t valid = KC ? (gr < rows ? (int64_t)K - gk : 0) : (gk < K ? (int64_t)rows - gr : 0);
+   return f8_border_chunk(mat + (KC ? gk + gr * ld : gr + gk * ld), valid, KC ? K : rows);
+}
+
 /* The chunks that a thread moves: threadIdx.x + THREADS i of every slab. They differ by whole rows (KC) or whole k (!KC)
    with the same twist. Rows that do not exist are never loaded: KC repeats the last row instead; !KC loads the last 16
    rows where a chunk passes the end, and moves them into place on the way to LDS (so `rows` is at least 16 there). What
@@ -103,13 +112,7 @@ template <bool KC, int R, int THREADS> struct F8Stage
       uint32_t thread = threadIdx.x;
       asm volatile("" : "+v"(thread));   /* what follows from it is computed here, not kept in registers through the pipelined slabs */
 #pragma unroll
-      for (int i = 0; i < NV; i++)
-      {  uint32_t row, k;
-         L::where(thread + THREADS * i, row, k);
-         const int64_t gr = (int64_t)r0 + row, gk = (int64_t)k0 + k;
-         const int64_t valid = KC ? (gr < rows ? (int64_t)K - gk : 0) : (gk < K ? (int64_t)rows - gr : 0);
-         v[i] = f8_border_chunk(mat + (KC ? gk + gr * ld : gr + gk * ld), valid, KC ? K : rows);
-      }
+      for (int i = 0; i < NV; i++) v[i] = f8_any_chunk<KC, R>(mat, ld, r0, k0, rows, K, thread + THREADS * i);
    }
    __device__ __forceinline__ void store(char *slab, bool border)
    {

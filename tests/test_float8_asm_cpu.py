@@ -8,7 +8,7 @@ import subprocess
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-SOURCES = ["och_gemm_f8_few_44.hip"]
+SOURCES = ["och_gemm_f8_few_44.hip", "och_gemm_f8_pipe_45.hip"]
 
 
 @pytest.mark.parametrize("source", SOURCES)
@@ -26,4 +26,4 @@ def test_m0_is_used_by_the_loads_to_lds_only(source, tmp_path):
     assert len(uses) >= 8, "no load to LDS found in %s" % source
     for i in uses:
         assert re.fullmatch(r"s_mov_b32 m0, s\d+", code[i]), code[i]
-        assert any(c.startswith("global_load_lds_dwordx4") for c in code[i + 1:i + 3]), code[i:i + 3]
+        assert any(c.startswith("global_load_lds_dword") for c in code[i + 1:i + 3]), code[i:i + 3]
