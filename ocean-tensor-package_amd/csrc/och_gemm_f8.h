@@ -84,6 +84,21 @@ template <bool E5A, bool E5B> __device__ __forceinline__ och_f32x4v f8_block(con
    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
    return c;
 }
+/* a row of TJ blocks; the wide instructions of two blocks alternate, because each needs the sums of the one before */
+template <bool E5A, bool E5B, int TJ> __device__ __forceinline__ void f8_row(const F8Operand<false> &a, const F8Operand<false> (&b)[TJ], och_f32x4v (&part)[TJ])
+{
+#pragma unroll
+   for (int j = 0; j < TJ; j++) part[j] = f8_block<E5A, E5B>(a, b[j]);
+}
+template <bool E5A, bool E5B, int TJ> __device__ __forceinline__ void f8_row(const F8Operand<true> &a, const F8Operand<true> (&b)[TJ], och_f32x4v (&part)[TJ])
+{  const och_f32x4v zero = { 0, 0, 0, 0 };
+   static_assert(TJ % 2 == 0, "pairs of blocks");
+#pragma unroll
+   for (int x = 0; x < 4 * TJ; x++)
+   {  const int j = x / 8 * 2 + x % 2, q = x / 2 % 4;
+      part[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b[j].v[q], q == 0 ? zero : part[j], 0, 0, 0);
+   }
+}
 
 /* the fragment of rows row0 .. + 15 (row0 a multiple of 16) of a slab in LDS */
 template <bool KC, int R> __device__ __forceinline__ och_i32x8 f8_fragment(const char *slab, uint32_t row0)

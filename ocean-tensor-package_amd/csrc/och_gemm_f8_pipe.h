@@ -2,14 +2,19 @@
  *
  * Eight waves, two per SIMD, own 128 x 64 of the tile each: 128 accumulator registers, so that the multiply-adds outside the
  * matrix cores (32 for every row of blocks) need no moves between register files, and a second wave on the SIMD whose
- * matrix instructions run beside them (bare loops: 1.7 PFLOP/s with one wave per SIMD, 3.4 with two, 4.1 without the
- * multiply-adds). The slab's 64 KB go from memory straight to LDS, one slab ahead of the matrix instructions, with one
- * barrier per slab: an element is loaded once per 256 of the other operand, half of what 128 x 128 tiles load. Row i of
- * blocks is multiplied while the fragment of row i + 1 is read and the sums of row i - 1 are scaled and added.
+ * matrix instructions run beside them. The slab's 64 KB go from memory straight to LDS: an element is loaded once per 256
+ * of the other operand, half of what 128 x 128 tiles load. Step i of a slab multiplies row i of blocks while the fragment of
+ * row i + 1 is read and the sums of row i - 1 are scaled and added. The one barrier of a slab stands in front of its last
+ * step, when the fragments of that step are in registers: behind it the next slab is complete, its first fragments are read
+ * during the last step, and this slab's buffer is free. The loads of the slab after the next go there, two or three to a
+ * step: a wave that issues all nine in a row waits for the memory pipe instead of multiplying (8192^3 on equal codes: 385 us,
+ * spread over a step each 405, two or three to a step 358, with the barrier and the first fragments moved into the last
+ * step 340).
  *
- * 8192^3 from e4m3 codes of Gaussian data to bfloat16: 480 us, 2.29 PFLOP/s; 384 us (2.86) when all codes are equal. The
- * difference is the power that changing operand bits draw, which is the bound: orders of the tiles, fragments read further
- * ahead or before the barrier, wave priorities and 32 x 32 x 64 instructions (8 % slower) change neither figure. */
+ * 8192^3 to bfloat16: 340 us, 3.24 PFLOP/s, when all codes are equal (bare loops of these matrix instructions and additions:
+ * 4.5 PFLOP/s on equal codes, 3.3 on changing ones), 465 us, 2.36 PFLOP/s, on random codes: what bounds it is the power that
+ * changing operand bits draw. Orders of the tiles, fragments read further ahead, wave priorities and two barriers with one
+ * and a half slabs in flight changed nothing or lost; 32 x 32 x 64 instructions are 8 % slower. */
 #pragma once
 #include "och_gemm_f8_tile.h"
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -99,64 +104,114 @@ __global__ __launch_bounds__(OCH_F8_PIPE_THREADS, 2) void gemm_f8_pipe_kernel(co
    const char *nextS = (const char *)((forA ? p.SA : p.SB) + (int64_t)scale_first * scale_line);
    const uint32_t scale_offset = (((line < most ? line : most) >> (forA ? p.shiftA : p.shiftB)) - scale_first) * (uint32_t)scale_line * 4;
    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-   auto fetch = [&](uint32_t buf)
+   const uint32_t whole = p.K / OCH_F8_SLAB, slabs = (p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB;
+   /* load x (0 .. 8) of slab s, which goes to buffer s mod 2 */
+   auto load = [&](int x, uint32_t s)
+   {  const uint32_t buf = lds0 + (s & 1) * BUF;
+      if (x < 8)
+      {  if (x % 2) lb.issue(x / 2, nextB, buf + OPERAND + 4096 * wave);
+         else       la.issue(x / 2, nextA, buf + 4096 * wave);
+      }
+      else
+      {  load_float_to_lds(nextS, scale_offset, buf + SCALES + 256 * wave);
+         nextA += stepA; nextB += stepB; nextS += scale_step;
+      }
+   };
+   /* the slab inside which K ends: chunk by chunk through registers (once per tile, not overlapped with anything) */
+   auto load_rest = [&]()
+   {  const uint32_t buf = (whole & 1) * BUF;
+      uint32_t q = threadIdx.x;
+      asm volatile("" : "+v"(q));                 /* nothing of this is worth a register in the loop */
+#pragma unroll 1
+      for (; q < F8Slab<AKC, R>::CHUNKS; q += THREADS)
+      {  const och_u32x4 va = f8_any_chunk<AKC, R>(p.A, p.ldA, m0, whole * OCH_F8_SLAB, p.M, p.K, q), vb = f8_any_chunk<BKC, R>(p.B, p.ldB, n0, whole * OCH_F8_SLAB, p.N, p.K, q);
+         *reinterpret_cast<och_u32x4 *>(lds + buf + 16 * q) = va;
+         *reinterpret_cast<och_u32x4 *>(lds + buf + OPERAND + 16 * q) = vb;
+      }
+      load_float_to_lds(nextS, scale_offset, lds0 + buf + SCALES + 256 * wave);
+   };
+   och_i32x8 a, b[TJ]; float ta = 1, t[TJ], told[TJ];            /* told: the slab before's */
+   och_f32x4v part[2][TJ], rs = zero;
+#pragma unroll
+   for (int j = 0; j < TJ; j++) { part[(TI - 1) % 2][j] = zero; told[j] = 0; }
+   auto scales_of = [&](const char *buf) { return reinterpret_cast<const float *>(buf + SCALES); };
+   auto column = [&](const char *buf, int j)
+   {  b[j] = f8_fragment<BKC, R>(buf + OPERAND, wn + 16 * j);
+      t[j] = scales_of(buf)[R + wn + 16 * j + lane % 16];
+   };
+   auto row_scales = [&](const char *buf, int i) { if (ROWS) rs = *reinterpret_cast<const och_f32x4v *>(scales_of(buf) + wm + 16 * i + 4 * (lane / 16)); };
+   auto multiply = [&](int i, int j, const och_i32x8 &now)
+   {  part[i % 2][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(now, b[j], zero, E5A ? 1 : 0, E5B ? 1 : 0, 0, 0, 0, 0); };
+   /* the sums of block (i, j), scaled; the empty statement keeps the addition where it is written */
+   auto add = [&](int i, int j, const float (&w)[TJ])
    {
 #pragma unroll
-      for (int e = 0; e < 4; e++) { la.issue(e, nextA, buf + 4096 * wave); lb.issue(e, nextB, buf + OPERAND + 4096 * wave); }
-      load_float_to_lds(nextS, scale_offset, buf + SCALES + 256 * wave);
-      nextA += stepA; nextB += stepB; nextS += scale_step;
+      for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf(part[i % 2][j][r], ROWS ? rs[r] * w[j] : w[j], acc[i][j][r]);
+      asm volatile("" : "+v"(acc[i][j]));
    };
-   const uint32_t whole = p.K / OCH_F8_SLAB, end = (p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB;
-   if (whole > 0) fetch(lds0);
-   for (uint32_t s = 0, turn = 0; s < end; s++, turn ^= 1)
-   {  char *buf = lds + turn * BUF;
-      const float *sA = reinterpret_cast<const float *>(buf + SCALES), *sB = sA + R;
-      if (s >= whole)
-      {  /* the rest of K, chunk by chunk through registers */
-         F8Stage<AKC, R, THREADS> ra; F8Stage<BKC, R, THREADS> rb;
-         __syncthreads();
-         ra.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); ra.store(buf, false);
-         rb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); rb.store(buf + OPERAND, false);
-         load_float_to_lds(nextS, scale_offset, lds0 + turn * BUF + SCALES + 256 * wave);
+   if (slabs > 0)
+   {  if (whole > 0)
+      {
+#pragma unroll
+         for (int x = 0; x < 9; x++) load(x, 0);
       }
+      else load_rest();
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (s + 1 < whole) fetch(lds0 + (turn ^ 1) * BUF);
-      och_i32x8 b[TJ]; float t[TJ];
+      if (whole > 1) { load(0, 1); load(1, 1); }
+      else if (slabs > 1) load_rest();
+      a = f8_fragment<AKC, R>(lds, wm);
+      if (!ROWS) ta = scales_of(lds)[wm];
 #pragma unroll
-      for (int j = 0; j < TJ; j++)
-      {  b[j] = f8_fragment<BKC, R>(buf + OPERAND, wn + 16 * j);
-         t[j] = sB[wn + 16 * j + lane % 16];
-         if (!ROWS) t[j] *= sA[wm];
-      }
-      och_i32x8 a = f8_fragment<AKC, R>(buf, wm);
-      och_f32x4v part[2][TJ], rs[2];
+      for (int j = 0; j < TJ; j++) column(lds, j);
+      for (uint32_t s = 0; s < slabs; s++)
+      {  const char *buf = lds + (s & 1) * BUF, *next = lds + ((s + 1) & 1) * BUF;
+         const bool more = s + 1 < whole;                      /* slab s + 1 is being loaded */
 #pragma unroll
-      for (int i = 0; i <= TI; i++)
-      {  if (i < TI)
+         for (int i = 0; i < TI - 1; i++)
          {  const och_i32x8 now = a;
-            if (i < TI - 1) a = f8_fragment<AKC, R>(buf, wm + 16 * (i + 1));
-            if (ROWS) rs[i % 2] = *reinterpret_cast<const och_f32x4v *>(sA + wm + 16 * i + 4 * (lane / 16));
+            if (more)
+            {  if (i == 0) { load(2, s + 1); load(3, s + 1); load(4, s + 1); }
+               if (i == 1) { load(5, s + 1); load(6, s + 1); }
+               if (i == 2) { load(7, s + 1); load(8, s + 1); }
+            }
+            a = f8_fragment<AKC, R>(buf, wm + 16 * (i + 1));
+            if (i > 0) row_scales(buf, i - 1);                 /* (row 0 finds those of the slab before's last row) */
 #pragma unroll
-            for (int j = 0; j < TJ; j++) part[i % 2][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(now, b[j], zero, E5A ? 1 : 0, E5B ? 1 : 0, 0, 0, 0, 0);
-         }
-         if (i > 0)
-         {  const int o = (i - 1) % 2, q = i > 0 ? i - 1 : 0;
+            for (int j = 0; j < TJ; j++) multiply(i, j, now);
 #pragma unroll
-            for (int j = 0; j < TJ; j++)
+            for (int j = 0; j < TJ; j++) { if (i == 0) add(TI - 1, j, told); else add(i > 0 ? i - 1 : 0, j, t); }
+            if (i == 0 && !ROWS)
+            {
 #pragma unroll
-               for (int r = 0; r < 4; r++) acc[q][j][r] = __builtin_fmaf(part[o][j][r], ROWS ? rs[o][r] * t[j] : t[j], acc[q][j][r]);
-#pragma unroll
-            for (int j = 0; j < TJ; j++) asm volatile("" : "+v"(acc[q][j]));
-         }
-         if (i > 0 && i < TI)
-         {
+               for (int j = 0; j < TJ; j++) t[j] *= ta;
+            }
 #pragma unroll
             for (int j = 0; j < TJ; j++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x2, ROWS ? 8 : 4, 0); }
+            __builtin_amdgcn_sched_barrier(0);
          }
-         __builtin_amdgcn_sched_barrier(0);
+         och_f32x4v last = zero;
+         if (ROWS) { row_scales(buf, TI - 1); last = rs; row_scales(buf, TI - 2); }
+         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+         __syncthreads();
+         if (s + 2 < whole) { load(0, s + 2); load(1, s + 2); }
+         else if (s + 2 == whole && slabs > whole) load_rest();
+         const och_i32x8 now = a;
+         a = f8_fragment<AKC, R>(next, wm);                    /* (behind the last slab: of no use, and none is made of it) */
+         if (!ROWS) ta = scales_of(next)[wm];
+#pragma unroll
+         for (int j = 0; j < TJ; j++)
+         {  multiply(TI - 1, j, now);
+            add(TI - 2, j, t);
+            told[j] = t[j];
+            column(next, j);
+            __builtin_amdgcn_sched_barrier(0);
+         }
+         rs = last;
       }
    }
+#pragma unroll
+   for (int j = 0; j < TJ; j++) add(TI - 1, j, told);
    /* C leaves through LDS, 128 columns at a time as floats with a pitch that spreads neighbouring columns over the banks, in
       pieces of eight rows: memory sees 512 consecutive bytes of a column */
    constexpr uint32_t PITCH = R * 4 + 16, HALF = 128;

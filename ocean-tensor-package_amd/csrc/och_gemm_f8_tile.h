@@ -71,29 +71,27 @@ template <bool KC, int R> static __device__ __forceinline__ och_u32x4 f8_any_chu
 template <bool KC, int R, int THREADS> struct F8Stage
 {
    typedef F8Slab<KC, R> L;
-   static constexpr int NV = (int)L::CHUNKS / THREADS, NP = KC ? NV : 1;
+   static constexpr int NV = (int)L::CHUNKS / THREADS;
    static constexpr uint32_t STEP = KC ? THREADS / 8 : THREADS / L::PER_K;       /* rows or k from a thread's chunk to its next */
    static_assert(STEP % 8 == 0, "the twist must not change from chunk to chunk");
    och_u32x4 v[NV];
-   const uint8_t *at[NP];
-   uint32_t move;
-   static __device__ __forceinline__ bool pipelined(uint32_t rows) { return KC || rows >= 16; }
+   const uint8_t *slab;                  /* the next slab's first element: the same for all threads */
+   uint32_t offset, most, move;          /* of the thread's first chunk from there, and (KC) of the same k of the last row; rows that a chunk is moved by */
+   /* offsets within a slab are counted in 32 bits */
+   static __device__ __forceinline__ bool pipelined(uint32_t rows, int64_t ld) { return (KC || rows >= 16) && ld < (1 << 24); }
    __device__ __forceinline__ void start(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows)
    {  uint32_t row, k;
       L::where(threadIdx.x, row, k);
-      if (KC)
-      {
-#pragma unroll
-         for (int i = 0; i < NP; i++)
-         {  const uint32_t r = r0 + row + i * STEP;
-            at[i] = mat + (int64_t)(k0 + k) + (int64_t)(r < rows ? r : rows - 1) * ld;
-         }
-         move = 0;
-      }
+      slab = mat + (KC ? (int64_t)k0 + (int64_t)r0 * ld : (int64_t)r0 + (int64_t)k0 * ld);
+      const uint32_t last = rows - r0 < R ? rows - r0 - 1 : R - 1;        /* the tile's last row */
+      move = 0;
+      most = last * (uint32_t)ld + k;
+      if (KC) offset = row * (uint32_t)ld + k;
       else
-      {  const uint32_t r = r0 + row, last = rows >= 16 ? rows - 16 : 0, from = r < last ? r : last;
-         at[0] = mat + from + (int64_t)(k0 + k) * ld;
-         move = r - from;
+      {  const int32_t from = (int32_t)row < (int32_t)last - 15 ? (int32_t)row : (int32_t)last - 15;      /* below zero: the chunk begins in front of the tile */
+         slab -= 16;
+         offset = (uint32_t)(from + 16) + k * (uint32_t)ld;
+         move = (uint32_t)((int32_t)row - from);
       }
    }
    /* the next slab, whole along k */
@@ -101,10 +99,10 @@ template <bool KC, int R, int THREADS> struct F8Stage
    {
 #pragma unroll
       for (int i = 0; i < NV; i++)
-      {  v[i] = *reinterpret_cast<const och_u32x4_any *>(KC ? at[i % NP] : at[0] + i * (int64_t)STEP * ld);
-         if (KC) at[i % NP] += OCH_F8_SLAB;
+      {  const uint32_t o = offset + i * STEP * (uint32_t)ld;
+         v[i] = *reinterpret_cast<const och_u32x4_any *>(KC ? slab + (o < most ? o : most) : slab + i * (int64_t)STEP * ld + offset);
       }
-      if (!KC) at[0] += OCH_F8_SLAB * ld;
+      slab += KC ? OCH_F8_SLAB : OCH_F8_SLAB * ld;
    }
    /* any slab, chunk by chunk */
    __device__ __forceinline__ void load_border(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows, uint32_t K)
@@ -150,34 +148,29 @@ template <int DT> __device__ __forceinline__ void f8_finish4(char *C, int64_t at
       for (int r = 0; r < 3; r++) if ((uint32_t)r < valid) f8_finish<DT>(C, at + r, s[r], alpha, beta);
    }
 }
-/* A wave's TI x TJ tiles of 16 x 16 to C: lane l holds rows 4 (l / 16) .. + 3 of column l mod 16 of every tile; m, n: this
-   lane's place in the first. One tile after the other (the fences), or the compiler keeps all addresses at once. */
-template <int DT, int TI, int TJ> __device__ __forceinline__ void f8_write(const F8GemmParams &p, uint32_t m, uint32_t n, const och_f32x4v (&acc)[TI][TJ])
+/* COLUMNS columns of R rows of sums from LDS (PITCH bytes from column to column) to C, eight rows of a column at a time: memory
+   sees runs of R elements */
+template <int DT, int R, uint32_t PITCH, uint32_t COLUMNS, int THREADS> __device__ __forceinline__ void f8_store_columns(const F8GemmParams &p, const char *lds, uint32_t m0, uint32_t n0)
 {
+   typedef typename Wide<DT>::E E;
+#pragma unroll 1
+   for (uint32_t q = threadIdx.x; q < COLUMNS * (R / 8); q += THREADS)
+   {  const uint32_t c = q / (R / 8), m = m0 + q % (R / 8) * 8, n = n0 + c;
+      if (m >= p.M || n >= p.N) continue;
+      const och_f32x4v *from = reinterpret_cast<const och_f32x4v *>(lds + c * PITCH + q % (R / 8) * 32);
+      const och_f32x4v lo = from[0], hi = from[1];
+      E *to = reinterpret_cast<E *>(p.C) + (int64_t)m + (int64_t)n * p.ldC;
+      const int64_t valid = (int64_t)p.M - m;
+      Wide8<DT> v;
+      if (p.beta != 0.0f) v.load(to, valid);
 #pragma unroll
-   for (int j = 0; j < TJ; j++)
-   {  if (n + 16 * j < p.N)
-      {  const int64_t column = (int64_t)(n + 16 * j) * p.ldC;
-#pragma unroll
-         for (int i = 0; i < TI; i++)
-            if (m + 16 * i < p.M) f8_finish4<DT>(p.C, column + m + 16 * i, acc[i][j], p.alpha, p.beta, p.M - m - 16 * i);
+      for (int e = 0; e < 8; e++)
+      {  float x = p.alpha * (e < 4 ? lo[e % 4] : hi[e % 4]);
+         if (p.beta != 0.0f) x = __builtin_fmaf(p.beta, v.get(e), x);
+         v.put(e, x);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      v.store(to, valid);
    }
-}
-/* ... or, for a share of K, as raw sums into the share's plane (M x N, dense) */
-template <int TI, int TJ> __device__ __forceinline__ void f8_write_share(const F8GemmParams &p, uint32_t share, uint32_t m, uint32_t n, const och_f32x4v (&acc)[TI][TJ])
-{
-   F8GemmParams q = p;
-   q.C = reinterpret_cast<char *>(p.partial + (size_t)share * p.M * p.N); q.ldC = p.M; q.alpha = 1.0f; q.beta = 0.0f;
-   f8_write<OCH_FLOAT, TI, TJ>(q, m, n, acc);
-}
-template <int TI, int TJ> __device__ __forceinline__ void f8_write_any(const F8GemmParams &p, uint32_t share, uint32_t m, uint32_t n, const och_f32x4v (&acc)[TI][TJ])
-{
-   if (p.share_slabs)              f8_write_share<TI, TJ>(p, share, m, n, acc);
-   else if (p.dtypeC == OCH_FLOAT) f8_write<OCH_FLOAT, TI, TJ>(p, m, n, acc);
-   else if (p.dtypeC == OCH_HALF)  f8_write<OCH_HALF, TI, TJ>(p, m, n, acc);
-   else                            f8_write<OCH_BFLOAT16, TI, TJ>(p, m, n, acc);
 }
 
 template <bool AKC, bool BKC, bool E5A, bool E5B, bool WIDE, bool ROWS>
@@ -200,14 +193,17 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
    uint32_t s = 0, end = all;
    if (p.share_slabs) { s = blockIdx.y * p.share_slabs; end = s + p.share_slabs < all ? s + p.share_slabs : all; }
 
-   /* every thread brings one scale: threads 0 .. 127 of A's rows, 128 .. 255 of B's columns; those outside C repeat the last */
-   const bool forA = threadIdx.x < R;
-   const uint32_t line = forA ? m0 + threadIdx.x : n0 + threadIdx.x - R, most = (forA ? p.M : p.N) - 1;
-   const float *scale = forA ? p.SA + (int64_t)((line < most ? line : most) >> p.shiftA) * p.sa_m : p.SB + (int64_t)((line < most ? line : most) >> p.shiftB) * p.sb_n;
-   const int64_t scale_step = forA ? p.sa_k : p.sb_k;
+   /* every thread brings one scale: waves 0 and 1 of A's rows, 2 and 3 of B's columns; those outside C repeat the last */
+   const bool forA = __builtin_amdgcn_readfirstlane(wave) < 2;
+   const uint32_t line = threadIdx.x % R, most = (forA ? p.M - m0 : p.N - n0) - 1, shift = forA ? p.shiftA : p.shiftB, begin = forA ? m0 : n0;
+   const uint32_t scale_of = ((begin + (line < most ? line : most)) >> shift) - (begin >> shift);
+   const int64_t scale_line = forA ? p.sa_m : p.sb_n, scale_step = forA ? p.sa_k : p.sb_k;
+   const float *scale = (forA ? p.SA : p.SB) + (int64_t)(begin >> shift) * scale_line + (int64_t)s * scale_step;
+   auto next_scale = [&]() { const float x = scale[(int64_t)scale_of * scale_line]; scale += scale_step; return x; };
 
-   /* slabs that are whole along k are pipelined; the rest of K, and everything of an operand of under 16 contiguous rows, is not */
-   const uint32_t whole = p.K / OCH_F8_SLAB, piped = !F8Stage<AKC, R, THREADS>::pipelined(p.M) || !F8Stage<BKC, R, THREADS>::pipelined(p.N) ? s : end < whole ? end : whole;
+   /* slabs that are whole along k are pipelined; the rest of K, and everything of an operand of under 16 contiguous rows or
+      of columns 16 MB apart, is not */
+   const uint32_t whole = p.K / OCH_F8_SLAB, piped = !F8Stage<AKC, R, THREADS>::pipelined(p.M, p.ldA) || !F8Stage<BKC, R, THREADS>::pipelined(p.N, p.ldB) ? s : end < whole ? end : whole;
    const bool borderA = m0 + R > p.M, borderB = n0 + R > p.N;
    F8Stage<AKC, R, THREADS> la; F8Stage<BKC, R, THREADS> lb; float ls = 0;
    la.start(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M); lb.start(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N);
@@ -216,7 +212,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
       reinterpret_cast<float *>(buf + 2 * OPERAND)[threadIdx.x] = ls;
    };
    if (s < piped)
-   {  la.load(p.ldA); lb.load(p.ldB); ls = scale[(int64_t)s * scale_step];
+   {  la.load(p.ldA); lb.load(p.ldB); ls = next_scale();
       stash(lds);
    }
    __syncthreads();
@@ -224,54 +220,81 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
    {  char *buf = lds + turn * BUF;
       const float *sA = reinterpret_cast<const float *>(buf + 2 * OPERAND), *sB = sA + R;
       if (s >= piped)
-      {  la.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); lb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); ls = scale[(int64_t)s * scale_step];
+      {  la.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); lb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); ls = next_scale();
          stash(buf);
          __syncthreads();
       }
       const bool more = s + 1 < piped;
-      if (more) { la.load(p.ldA); lb.load(p.ldB); ls = scale[(int64_t)(s + 1) * scale_step]; }
+      if (more) { la.load(p.ldA); lb.load(p.ldB); ls = next_scale(); }
       F8Operand<WIDE> b[4]; float t[4];
+      {  och_i32x8 c[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-      {  b[j].template set<E5B>(f8_fragment<BKC, R>(buf + OPERAND, wn + 16 * j));
-         t[j] = sB[wn + 16 * j + lane % 16];
-         if (!ROWS) t[j] *= sA[wm];
+         for (int j = 0; j < 4; j++) { c[j] = f8_fragment<BKC, R>(buf + OPERAND, wn + 16 * j); t[j] = sB[wn + 16 * j + lane % 16]; }
+         const float whole_a = ROWS ? 1.0f : sA[wm];
          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+         for (int j = 0; j < 4; j++)
+         {  b[j].template set<E5B>(c[j]);
+            if (!ROWS) t[j] *= whole_a;
+            __builtin_amdgcn_sched_barrier(0);
+         }
       }
-      /* step i: the fragment of row i + 1 is read, row i multiplied, the sums of row i - 1 scaled and added; the fences keep
-         the compiler from collecting more rows' sums than registers hold */
-      och_i32x8 codes = f8_fragment<AKC, R>(buf, wm);
-      och_f32x4v part[2][4], rs[2];
+      /* step i: row i is multiplied while the sums of row i - 1 are scaled and added and the fragment of row i + 1 is read
+         and made an operand. The fences keep the compiler from collecting more rows than registers hold. */
+      F8Operand<WIDE> a;
+      a.template set<E5A>(f8_fragment<AKC, R>(buf, wm));
+      och_f32x4v part[2][4];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i <= 4; i++)
-      {  if (i < 4)
-         {  F8Operand<WIDE> a;
-            a.template set<E5A>(codes);
-            if (i < 3) codes = f8_fragment<AKC, R>(buf, wm + 16 * (i + 1));
-            if (ROWS) rs[i % 2] = *reinterpret_cast<const och_f32x4v *>(sA + wm + 16 * i + 4 * (lane / 16));
-#pragma unroll
-            for (int j = 0; j < 4; j++) part[i % 2][j] = f8_block<E5A, E5B>(a, b[j]);
-         }
+      {  och_i32x8 codes; F8Operand<WIDE> next = a; och_f32x4v rs;
+         if (ROWS && i > 0) rs = *reinterpret_cast<const och_f32x4v *>(sA + wm + 16 * (i > 0 ? i - 1 : 0) + 4 * (lane / 16));
+         if (i < 3) codes = f8_fragment<AKC, R>(buf, wm + 16 * (i + 1));
+         if (i < 4)
+            f8_row<E5A, E5B, 4>(a, b, part[i % 2]);
          if (i > 0)
-         {  const int o = (i - 1) % 2;
+         {  const int o = (i - 1) % 2, q = i > 0 ? i - 1 : 0;
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
-               for (int r = 0; r < 4; r++) acc[i > 0 ? i - 1 : 0][j][r] = __builtin_fmaf(part[o][j][r], ROWS ? rs[o][r] * t[j] : t[j], acc[i > 0 ? i - 1 : 0][j][r]);
+               for (int r = 0; r < 4; r++) acc[q][j][r] = __builtin_fmaf(part[o][j][r], ROWS ? rs[r] * t[j] : t[j], acc[q][j][r]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) asm volatile("" : "+v"(acc[i > 0 ? i - 1 : 0][j]));      /* here, not behind the loop's last branch */
+            for (int j = 0; j < 4; j++) asm volatile("" : "+v"(acc[q][j]));      /* here, not behind the loop's last branch */
          }
-         if (i > 0 && i < 4)
-         {  /* one block's matrix instructions, then the additions of a block of the row before */
+         if (i < 3) next.template set<E5A>(codes);
+         if (i < 4)
+         {  /* matrix instructions and the vector instructions of their time in turn */
+            constexpr int N = WIDE ? 16 : 4;
 #pragma unroll
-            for (int j = 0; j < 4; j++) { __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 1, 0); __builtin_amdgcn_sched_group_barrier(0x2, ROWS ? 8 : 4, 0); }
+            for (int x = 0; x < N; x++)
+            {  __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+               __builtin_amdgcn_sched_group_barrier(0x2, WIDE ? (ROWS ? 3 : 2) : (ROWS ? 8 : 4), 0);
+            }
          }
+         a = next;
          __builtin_amdgcn_sched_barrier(0);
       }
       if (more) stash(lds + (turn ^ 1) * BUF);
       __syncthreads();
    }
-   f8_write_any<4, 4>(p, blockIdx.y, m0 + wm + 4 * (lane / 16), n0 + wn + lane % 16, acc);
+   /* the tile leaves through LDS, where the slabs were; a share of K as raw sums into the share's plane (M x N, dense) */
+   constexpr uint32_t PITCH = R * 4 + 16;
+   static_assert(R * PITCH <= 2 * BUF, "the tile fits where the slabs were");
+   {  char *mine = lds + (wn + lane % 16) * PITCH + (wm + 4 * (lane / 16)) * 4;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+         for (int i = 0; i < 4; i++) *reinterpret_cast<och_f32x4v *>(mine + 16 * j * PITCH + 64 * i) = acc[i][j];
+   }
+   __syncthreads();
+   if (p.share_slabs)
+   {  F8GemmParams q = p;
+      q.C = reinterpret_cast<char *>(p.partial + (size_t)blockIdx.y * p.M * p.N); q.ldC = p.M; q.alpha = 1.0f; q.beta = 0.0f;
+      f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS>(q, lds, m0, n0);
+   }
+   else if (WIDE)                 f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS>(p, lds, m0, n0);
+   else if (p.dtypeC == OCH_HALF) f8_store_columns<OCH_HALF, R, PITCH, R, THREADS>(p, lds, m0, n0);
+   else                           f8_store_columns<OCH_BFLOAT16, R, PITCH, R, THREADS>(p, lds, m0, n0);
 }
 
 template <bool E5A, bool E5B, bool WIDE, bool ROWS> static int gemm_f8_tile_launch(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream)
