@@ -13,6 +13,7 @@
 namespace och {
 
 #define OCH_NORM_THREADS 256
+#define OCH_NORM_LONG (OCH_NORM_THREADS * 8 * 8)      /* longest row that stays in registers */
 
 /* x of the lane that the DPP control names, added */
 template <int CTRL> __device__ __forceinline__ float dpp_add(float x)
@@ -34,6 +35,13 @@ __device__ __forceinline__ float block_sum(float x, float *part)
    for (unsigned w = 0; w < blockDim.x / 64; w++) s += part[w];
    __syncthreads();
    return s;
+}
+
+/* sum over the T threads that share a row (T a power of two from 16 on; BLOCK threads in all) */
+template <int T> __device__ __forceinline__ float group_sum(float x, float *part)
+{  if (T == 16) return row16_sum(x);
+   if (T == 64) return wave64_sum(x);
+   return block_sum(x, part);
 }
 
 struct NormParams
@@ -126,9 +134,71 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_long_kernel(const NormP
    }
 }
 
+/* Rows of at most 8 T V elements: T threads keep a row in registers, eight neighbouring elements in each of V vectors per
+   thread, OCH_NORM_THREADS / T rows per workgroup. One pass over memory, which is what bounds it. */
+template <int DT, int CODE, int T, int V>
+__global__ __launch_bounds__(OCH_NORM_THREADS) void norm_kernel(const NormParams p)
+{
+   typedef typename Wide<DT>::E E;
+   __shared__ float part[OCH_NORM_THREADS / 64];
+   const int64_t wanted = (int64_t)blockIdx.x * (OCH_NORM_THREADS / T) + threadIdx.x / T;
+   const bool live = wanted < p.rows;
+   const int64_t row = live ? wanted : p.rows - 1;
+   const int first = (int)(threadIdx.x % T) * 8, n = live ? (int)p.n : 0;      /* a group without a row: no element is valid */
+   const E *x = reinterpret_cast<const E *>(p.X) + row * p.ldX;
+   Wide8<DT> h[V];
+#pragma unroll
+   for (int v = 0; v < V; v++) h[v].load(x + first + v * T * 8, n - first - v * T * 8);
+   if (p.R)
+   {  const E *r = reinterpret_cast<const E *>(p.R) + row * p.ldR;
+      Wide8<DT> a[V];
+#pragma unroll
+      for (int v = 0; v < V; v++) a[v].load(r + first + v * T * 8, n - first - v * T * 8);
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+         for (int e = 0; e < 8; e++) h[v].put(e, h[v].get(e) + a[v].get(e));
+   }
+   if (p.H)
+   {  E *to = reinterpret_cast<E *>(p.H) + row * p.ldH;
+#pragma unroll
+      for (int v = 0; v < V; v++) h[v].store(to + first + v * T * 8, n - first - v * T * 8);
+   }
+   float sum = 0;
+#pragma unroll
+   for (int v = 0; v < V; v++)
+   {  float s = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) s = __builtin_fmaf(h[v].get(e), h[v].get(e), s);
+      sum += s;
+   }
+   const float rstd = 1.0f / sqrtf(group_sum<T>(sum, part) / (float)p.n + p.eps);
+   if (p.rstd && live && threadIdx.x % T == 0) p.rstd[row] = rstd;
+#pragma unroll
+   for (int v = 0; v < V; v++)
+   {  const int at = first + v * T * 8;
+      float w[8], y[8];
+      load_weights<DT>(p.W, p.w_float, at, n - at, w);
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = h[v].get(e) * rstd * w[e];
+      norm_store<DT, CODE>(p, row, at, n - at, y);
+   }
+}
+
 template <int DT, int CODE> static int norm_launch(const NormParams &p, hipStream_t stream)
 {
-   hipLaunchKernelGGL((norm_long_kernel<DT, CODE>), dim3((unsigned)p.rows), dim3(OCH_NORM_THREADS), 0, stream, p);
+#define OCH_GO(T, V) hipLaunchKernelGGL((norm_kernel<DT, CODE, T, V>), dim3((unsigned)((p.rows + OCH_NORM_THREADS / T - 1) / (OCH_NORM_THREADS / T))), dim3(OCH_NORM_THREADS), 0, stream, p)
+   if (p.n <= 128)        OCH_GO(16, 1);
+   else if (p.n <= 256)   OCH_GO(16, 2);
+   else if (p.n <= 512)   OCH_GO(64, 1);
+   else if (p.n <= 1024)  OCH_GO(64, 2);
+   else if (p.n <= 2048)  OCH_GO(256, 1);
+   else if (p.n <= 4096)  OCH_GO(256, 2);
+   else if (p.n <= 6144)  OCH_GO(256, 3);
+   else if (p.n <= 8192)  OCH_GO(256, 4);
+   else if (p.n <= OCH_NORM_LONG) OCH_GO(256, 8);
+   else hipLaunchKernelGGL((norm_long_kernel<DT, CODE>), dim3((unsigned)p.rows), dim3(OCH_NORM_THREADS), 0, stream, p);
+#undef OCH_GO
    OCH_CHECK_LAUNCH();
    return 0;
 }
@@ -189,20 +259,121 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_long_kernel(const 
    }
 }
 
-/* dw: the workgroups' sums, added in their order */
-__global__ __launch_bounds__(256) void norm_grad_finish_kernel(const float *partial, int64_t n, uint32_t groups, float *dW)
+/* Rows of at most 8 T V elements: T threads keep a row in registers; a workgroup takes OCH_NORM_THREADS / T rows at a time,
+   in steps of the grid, and its threads' sums for dw stay in registers until its last row. T = 64: the four waves' sums meet
+   in LDS then. */
+template <int DT, int T, int V>
+__global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_kernel(const NormGradParams p)
 {
-   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-   if (at >= n) return;
+   typedef typename Wide<DT>::E E;
+   constexpr int ROWS = OCH_NORM_THREADS / T;
+   __shared__ float part[OCH_NORM_THREADS / 64];
+   __shared__ __align__(16) float meet[ROWS > 1 ? ROWS * T * V * 8 : 4];
+   const int first = (int)(threadIdx.x % T) * 8, n = (int)p.n;
+   float w[V][8], dw[V][8];
+#pragma unroll
+   for (int v = 0; v < V; v++)
+   {  load_weights<DT>(p.W, p.w_float, first + v * T * 8, n - first - v * T * 8, w[v]);
+#pragma unroll
+      for (int e = 0; e < 8; e++) dw[v][e] = 0;
+   }
+   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.rows; row0 += (int64_t)gridDim.x * ROWS)
+   {  const int64_t wanted = row0 + threadIdx.x / T;
+      const bool live = wanted < p.rows;
+      const int64_t row = live ? wanted : p.rows - 1;
+      const int valid = live ? n : 0;
+      Wide8<DT> a[V], b[V], c[V];
+#pragma unroll
+      for (int v = 0; v < V; v++)
+      {  const int at = first + v * T * 8;
+         a[v].load(reinterpret_cast<const E *>(p.dY) + row * p.lddY + at, valid - at);
+         b[v].load(reinterpret_cast<const E *>(p.H) + row * p.ldH + at, valid - at);
+         if (p.dH) c[v].load(reinterpret_cast<const E *>(p.dH) + row * p.lddH + at, valid - at);
+      }
+      const float rstd = p.rstd[row];
+      float sum = 0;
+#pragma unroll
+      for (int v = 0; v < V; v++)
+      {  float s = 0;
+#pragma unroll
+         for (int e = 0; e < 8; e++) s = __builtin_fmaf(a[v].get(e) * w[v][e], b[v].get(e) * rstd, s);
+         sum += s;
+      }
+      const float mean = group_sum<T>(sum, part) / (float)p.n;
+#pragma unroll
+      for (int v = 0; v < V; v++)
+      {  const int at = first + v * T * 8;
+         Wide8<DT> o;
+#pragma unroll
+         for (int e = 0; e < 8; e++)
+         {  const float u = b[v].get(e) * rstd;
+            float x = rstd * (a[v].get(e) * w[v][e] - u * mean);
+            if (p.dH) x += c[v].get(e);
+            o.put(e, x);
+            dw[v][e] = __builtin_fmaf(a[v].get(e), live ? u : 0.0f, dw[v][e]);
+         }
+         o.store(reinterpret_cast<E *>(p.dX) + row * p.lddX + at, valid - at);
+      }
+   }
+   if (p.partial == nullptr) return;
+   if (ROWS > 1)
+   {  float *mine = meet + threadIdx.x / T * (T * V * 8);
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+         for (int e = 0; e < 8; e++) mine[first + v * T * 8 + e] = dw[v][e];
+      __syncthreads();
+      if (threadIdx.x >= T) return;
+#pragma unroll
+      for (int v = 0; v < V; v++)
+#pragma unroll
+         for (int e = 0; e < 8; e++)
+         {  float s = 0;
+            for (int g = 0; g < ROWS; g++) s += meet[g * (T * V * 8) + first + v * T * 8 + e];
+            dw[v][e] = s;
+         }
+   }
+   float *to = p.partial + (int64_t)blockIdx.x * p.n;
+#pragma unroll
+   for (int v = 0; v < V; v++)
+   {  Wide8<OCH_FLOAT> d;
+#pragma unroll
+      for (int e = 0; e < 8; e++) d.put(e, dw[v][e]);
+      d.store(to + first + v * T * 8, n - first - v * T * 8);
+   }
+}
+
+/* dw: the workgroups' sums, added in a fixed order: sixteen threads per column take every sixteenth workgroup, their sums
+   meet in LDS */
+__global__ __launch_bounds__(1024) void norm_grad_finish_kernel(const float *partial, int64_t n, uint32_t groups, float *dW)
+{
+   __shared__ float meet[16][64];
+   const uint32_t lane = threadIdx.x % 64, slice = threadIdx.x / 64;
+   const int64_t at = (int64_t)blockIdx.x * 64 + lane;
    float s = 0;
-   for (uint32_t g = 0; g < groups; g++) s += partial[(int64_t)g * n + at];
+   if (at < n)
+   {  uint32_t g = slice;
+      for (; g + 7 * 16 < groups; g += 8 * 16)
+      {  float v[8];
+#pragma unroll
+         for (int u = 0; u < 8; u++) v[u] = partial[(int64_t)(g + 16 * u) * n + at];
+#pragma unroll
+         for (int u = 0; u < 8; u++) s += v[u];
+      }
+      for (; g < groups; g += 16) s += partial[(int64_t)g * n + at];
+   }
+   meet[slice][lane] = s;
+   __syncthreads();
+   if (slice != 0 || at >= n) return;
+   for (int k = 1; k < 16; k++) s += meet[k][lane];
    dW[at] = s;
 }
 
 template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipStream_t stream)
 {
-   uint64_t groups = 2 * (uint64_t)gemm_compute_units();
-   if (groups > (uint64_t)p.rows) groups = (uint64_t)p.rows;
+   const int rows_at_once = p.n <= 1024 ? 4 : 1;
+   uint64_t groups = 4 * (uint64_t)gemm_compute_units();
+   if (groups > ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once) groups = ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once;
    p.partial = nullptr;
    if (dW)
    {  const uint64_t fit = OCH_GEMM_WORKSPACE / ((uint64_t)p.n * sizeof(float));
@@ -212,10 +383,18 @@ template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipSt
       if (stream_gemm_workspace(stream, &ws) != 0) return -1;
       p.partial = reinterpret_cast<float *>(ws);
    }
-   hipLaunchKernelGGL((norm_grad_long_kernel<DT>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p);
+#define OCH_GO(T, V) hipLaunchKernelGGL((norm_grad_kernel<DT, T, V>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p)
+   if (p.n <= 512)        OCH_GO(64, 1);
+   else if (p.n <= 1024)  OCH_GO(64, 2);
+   else if (p.n <= 2048)  OCH_GO(256, 1);
+   else if (p.n <= 4096)  OCH_GO(256, 2);
+   else if (p.n <= 6144)  OCH_GO(256, 3);
+   else if (p.n <= 8192)  OCH_GO(256, 4);
+   else hipLaunchKernelGGL((norm_grad_long_kernel<DT>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p);
+#undef OCH_GO
    OCH_CHECK_LAUNCH();
    if (dW)
-   {  hipLaunchKernelGGL(norm_grad_finish_kernel, dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, stream, p.partial, p.n, (uint32_t)groups, dW);
+   {  hipLaunchKernelGGL(norm_grad_finish_kernel, dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, p.partial, p.n, (uint32_t)groups, dW);
       OCH_CHECK_LAUNCH();
    }
    return 0;
