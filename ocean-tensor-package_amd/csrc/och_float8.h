@@ -77,33 +77,59 @@ __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b 
 
 /* largest value over the row of 16 lanes, in all of its lanes */
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t x)
-{  return umax(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, false)); }
+{  return umax(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true)); }
 __device__ __forceinline__ uint32_t row16_max(uint32_t x)
 {  x = dpp_max<0xB1>(x); x = dpp_max<0x4E>(x); x = dpp_max<0x141>(x); return dpp_max<0x140>(x); }
+
+/* Largest magnitudes of elements as they lie in memory, word by word: one float or two 16-bit elements in a word, which are
+   compared without being converted */
+typedef unsigned short och_u16x2 __attribute__((ext_vector_type(2)));
+template <int DT> __device__ __forceinline__ uint32_t word_magnitude(uint32_t w) { return w & (DT == OCH_FLOAT ? 0x7FFFFFFFu : 0x7FFF7FFFu); }
+template <int DT> __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b)
+{  if (DT == OCH_FLOAT) return umax(a, b);
+   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(och_u16x2, a), __builtin_bit_cast(och_u16x2, b)));
+}
+/* element i of the word, as the bits of a float */
+template <int DT> __device__ __forceinline__ uint32_t word_float_bits(uint32_t w, int i)
+{  if constexpr (DT == OCH_FLOAT) return w;
+   else return __float_as_uint(Wide<DT>::get(__builtin_bit_cast(typename Wide<DT>::E, (unsigned short)(w >> 16 * i))));
+}
 
 template <int CODE> struct Code8 { static constexpr float MOST = (CODE == OCH_FLOAT8_E4M3) ? 448.0f : 57344.0f; };
 
 /* scale and factor of a block by the bits of its largest magnitude: values are multiplied by the factor before they are
    rounded to codes, codes times the scale give the values back. Magnitudes below 2^-100 count as 2^-100, which keeps both
-   numbers finite and normal; a block that holds an infinity or a NaN gets scale NaN. */
+   numbers finite and normal; a block that holds an infinity or a NaN gets scale NaN.
+
+   Both quotients are correctly rounded, in far fewer instructions than a general division takes, whose cases (subnormal
+   numbers, overflow, zero) cannot occur: a quotient by a reciprocal, and one correction by its exact remainder (Markstein,
+   IBM J. Res. Dev. 34, 1990). a 2^-20 keeps the reciprocal normal for every a. All 2^23 significands of a were compared with
+   the division for both types; powers of two scale every step exactly. */
 template <int CODE> __device__ __forceinline__ void block_scale(uint32_t largest, float &scale, float &factor, bool &bad)
-{  bad = largest >= 0x7F800000u;
+{  constexpr float MOST = Code8<CODE>::MOST, INVERSE = 1.0f / MOST, SMALL = 0x1p-20f;
+   bad = largest >= 0x7F800000u;
    const float a = fmaxf(__uint_as_float(largest), 0x1p-100f);
-   scale = bad ? __uint_as_float(0x7FC00000u) : a / Code8<CODE>::MOST;
-   factor = Code8<CODE>::MOST / a;
+   float q = a * INVERSE;
+   q = __builtin_fmaf(__builtin_fmaf(-MOST, q, a), INVERSE, q);
+   scale = bad ? __uint_as_float(0x7FC00000u) : q;
+   const float d = a * SMALL;
+   float r = __builtin_amdgcn_rcpf(d);
+   r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+   q = (MOST * SMALL) * r;
+   factor = __builtin_fmaf(__builtin_fmaf(-d, q, MOST * SMALL), r, q);
 }
 
-/* four codes, round to nearest even. The product with the factor can pass the largest code by one rounding: the clamp
-   keeps it there, because what the conversion makes of larger values depends on a mode bit */
-template <int CODE> __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float factor, bool bad)
-{  constexpr float M = Code8<CODE>::MOST;
-   a = __builtin_amdgcn_fmed3f(a * factor, -M, M); b = __builtin_amdgcn_fmed3f(b * factor, -M, M);
-   c = __builtin_amdgcn_fmed3f(c * factor, -M, M); d = __builtin_amdgcn_fmed3f(d * factor, -M, M);
-   int r = 0;
+/* four codes of values that are multiplied by their factors, round to nearest even. The product can pass the largest code by one rounding, from where the
+   conversion comes back to the largest code: what it rounds to, not what it is given, decides about overflow */
+template <int CODE> __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d)
+{  int r = 0;
    if (CODE == OCH_FLOAT8_E4M3) { r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false); r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true); }
    else                         { r = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, r, false); r = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, r, true); }
-   return bad ? 0x7F7F7F7Fu : (uint32_t)r;            /* 0x7F is a NaN of both code types */
+   return (uint32_t)r;
 }
+/* the same with one factor; a block with an infinity or a NaN is 0x7F throughout, a NaN of both code types */
+template <int CODE> __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float factor, bool bad)
+{  return bad ? 0x7F7F7F7Fu : code4<CODE>(a * factor, b * factor, c * factor, d * factor); }
 
 /* eight codes to memory, the first `valid` of them */
 __device__ __forceinline__ void store_codes(uint8_t *at, och_u32x2 q, int64_t valid)

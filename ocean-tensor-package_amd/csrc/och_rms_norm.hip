@@ -13,11 +13,10 @@
 namespace och {
 
 #define OCH_NORM_THREADS 256
-#define OCH_NORM_LONG (OCH_NORM_THREADS * 8 * 8)      /* longest row that stays in registers */
 
 /* x of the lane that the DPP control names, added */
 template <int CTRL> __device__ __forceinline__ float dpp_add(float x)
-{  const int i = __float_as_int(x); return x + __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false)); }
+{  const int i = __float_as_int(x); return x + __int_as_float(__builtin_amdgcn_update_dpp(0, i, CTRL, 0xF, 0xF, true)); }
 __device__ __forceinline__ float row16_sum(float x)
 {  x = dpp_add<0xB1>(x); x = dpp_add<0x4E>(x); x = dpp_add<0x141>(x); return dpp_add<0x140>(x); }
 __device__ __forceinline__ float lane_float(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
@@ -44,14 +43,25 @@ template <int T> __device__ __forceinline__ float group_sum(float x, float *part
    return block_sum(x, part);
 }
 
+/* rows that a workgroup holds at a time when T threads share one */
+constexpr int norm_rows(int T) { return T < OCH_NORM_THREADS ? OCH_NORM_THREADS / T : 1; }
+
 struct NormParams
 {
    const char *X, *R, *W; char *H, *Y; float *S, *rstd;
    int64_t  ldX, ldR, ldH, ldY, ldS;    /* in elements */
    int64_t  n, rows;
-   float    eps;
+   float    eps, inverse;               /* inverse: 1 / n */
    int      w_float;                    /* the weights are float (else the type of X) */
 };
+
+/* 1 / sqrt(x): the instruction's result and one step of Newton's method; where that could leave the range of normal numbers,
+   root and division */
+__device__ __forceinline__ float inverse_root(float x)
+{  if (!(x >= 0x1p-100f && x <= 0x1p100f)) return 1.0f / sqrtf(x);
+   const float r = __builtin_amdgcn_rsqf(x);
+   return __builtin_fmaf(0.5f * r, __builtin_fmaf(-x * r, r, 1.0f), r);
+}
 
 /* eight weights as floats (1 when there are none) */
 template <int DT> __device__ __forceinline__ void load_weights(const char *W, int w_float, int64_t at, int64_t valid, float *w)
@@ -83,11 +93,11 @@ template <int DT, int CODE> __device__ __forceinline__ void norm_store(const Nor
       o.store(reinterpret_cast<typename Wide<DT>::E *>(p.Y) + at + row * p.ldY, valid);
    }
    else
-   {  uint32_t m = 0;
+   {  float m = 0;                                        /* a NaN stays; values behind the row's end are zero, or NaN with the row */
 #pragma unroll
-      for (int e = 0; e < 8; e++) m = umax(m, e < valid ? magnitude_bits(y[e]) : 0u);
+      for (int e = 0; e < 8; e++) m = __builtin_elementwise_maximum(m, fabsf(y[e]));
       float scale, factor; bool bad;
-      block_scale<CODE>(row16_max(m), scale, factor, bad);
+      block_scale<CODE>(row16_max(magnitude_bits(m)), scale, factor, bad);
       och_u32x2 q;
       q.x = code4<CODE>(y[0], y[1], y[2], y[3], factor, bad);
       q.y = code4<CODE>(y[4], y[5], y[6], y[7], factor, bad);
@@ -120,7 +130,7 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_long_kernel(const NormP
       for (int e = 0; e < 8; e++) s = __builtin_fmaf(v.get(e), v.get(e), s);
       sum += s;
    }
-   const float rstd = 1.0f / sqrtf(block_sum(sum, part) / (float)p.n + p.eps);
+   const float rstd = inverse_root(block_sum(sum, part) * p.inverse + p.eps);
    if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
    const E *again = p.H ? h : x;                           /* every thread reads what it wrote or read itself */
    for (int64_t at0 = 0; at0 < p.n; at0 += OCH_NORM_THREADS * 8)
@@ -135,13 +145,15 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_long_kernel(const NormP
 }
 
 /* Rows of at most 8 T V elements: T threads keep a row in registers, eight neighbouring elements in each of V vectors per
-   thread, OCH_NORM_THREADS / T rows per workgroup. One pass over memory, which is what bounds it. */
+   thread, norm_rows(T) rows per workgroup. One pass over memory, which is what bounds it, then the instructions per element: with a
+   general division for scale, factor, mean and root, 8192 rows of 8192 bfloat16 features to codes took 47.4 us, now 42.8.
+   With the residual stream in and out: 84.3 us (5.6 TB/s of reads and writes); 5003 float features: 5.2 TB/s. */
 template <int DT, int CODE, int T, int V>
-__global__ __launch_bounds__(OCH_NORM_THREADS) void norm_kernel(const NormParams p)
+__global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams p)
 {
    typedef typename Wide<DT>::E E;
-   __shared__ float part[OCH_NORM_THREADS / 64];
-   const int64_t wanted = (int64_t)blockIdx.x * (OCH_NORM_THREADS / T) + threadIdx.x / T;
+   __shared__ float part[T * norm_rows(T) / 64];
+   const int64_t wanted = (int64_t)blockIdx.x * norm_rows(T) + threadIdx.x / T;
    const bool live = wanted < p.rows;
    const int64_t row = live ? wanted : p.rows - 1;
    const int first = (int)(threadIdx.x % T) * 8, n = live ? (int)p.n : 0;      /* a group without a row: no element is valid */
@@ -172,7 +184,7 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_kernel(const NormParams
       for (int e = 0; e < 8; e++) s = __builtin_fmaf(h[v].get(e), h[v].get(e), s);
       sum += s;
    }
-   const float rstd = 1.0f / sqrtf(group_sum<T>(sum, part) / (float)p.n + p.eps);
+   const float rstd = inverse_root(group_sum<T>(sum, part) * p.inverse + p.eps);
    if (p.rstd && live && threadIdx.x % T == 0) p.rstd[row] = rstd;
 #pragma unroll
    for (int v = 0; v < V; v++)
@@ -185,9 +197,13 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_kernel(const NormParams
    }
 }
 
+/* Threads and vectors by the row's length: as few threads as hold the row in two vectors each, because a group within a wave
+   needs no barrier, but from there on more threads than vectors. 2^26 bfloat16 values with the residual stream, to codes:
+      8192 features: 512 threads x 2 vectors 86.0 us, 256 x 4 90.2, 64 x 16 far behind;   16384: 512 x 4 91 us, 256 x 8 101;
+      4096: 256 x 2 84.9 us, 512 x 1 83.4, but 48 against 58 without the residual stream;   5003 float: 256 x 3 15.3, 512 x 2 16.7 */
 template <int DT, int CODE> static int norm_launch(const NormParams &p, hipStream_t stream)
 {
-#define OCH_GO(T, V) hipLaunchKernelGGL((norm_kernel<DT, CODE, T, V>), dim3((unsigned)((p.rows + OCH_NORM_THREADS / T - 1) / (OCH_NORM_THREADS / T))), dim3(OCH_NORM_THREADS), 0, stream, p)
+#define OCH_GO(T, V) hipLaunchKernelGGL((norm_kernel<DT, CODE, T, V>), dim3((unsigned)((p.rows + norm_rows(T) - 1) / norm_rows(T))), dim3(T * norm_rows(T)), 0, stream, p)
    if (p.n <= 128)        OCH_GO(16, 1);
    else if (p.n <= 256)   OCH_GO(16, 2);
    else if (p.n <= 512)   OCH_GO(64, 1);
@@ -195,8 +211,8 @@ template <int DT, int CODE> static int norm_launch(const NormParams &p, hipStrea
    else if (p.n <= 2048)  OCH_GO(256, 1);
    else if (p.n <= 4096)  OCH_GO(256, 2);
    else if (p.n <= 6144)  OCH_GO(256, 3);
-   else if (p.n <= 8192)  OCH_GO(256, 4);
-   else if (p.n <= OCH_NORM_LONG) OCH_GO(256, 8);
+   else if (p.n <= 8192)  OCH_GO(512, 2);
+   else if (p.n <= 16384) OCH_GO(512, 4);
    else hipLaunchKernelGGL((norm_long_kernel<DT, CODE>), dim3((unsigned)p.rows), dim3(OCH_NORM_THREADS), 0, stream, p);
 #undef OCH_GO
    OCH_CHECK_LAUNCH();
@@ -209,6 +225,7 @@ struct NormGradParams
    const char *dY, *H, *W, *dH; char *dX; const float *rstd; float *partial;   /* partial: n sums per workgroup, null when dW is not asked for */
    int64_t  lddY, ldH, lddH, lddX;
    int64_t  n, rows;
+   float    inverse;                    /* 1 / n */
    int      w_float;
 };
 
@@ -232,7 +249,7 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_long_kernel(const 
          for (int e = 0; e < 8; e++) s = __builtin_fmaf(a.get(e) * w[e], b.get(e) * rstd, s);
          sum += s;
       }
-      const float mean = block_sum(sum, part) / (float)p.n;
+      const float mean = block_sum(sum, part) * p.inverse;
       for (int64_t at = threadIdx.x * 8; at < p.n; at += OCH_NORM_THREADS * 8)
       {  Wide8<DT> a, b, c, o; Wide8<OCH_FLOAT> d; float w[8];
          const int64_t valid = p.n - at;
@@ -259,15 +276,15 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_long_kernel(const 
    }
 }
 
-/* Rows of at most 8 T V elements: T threads keep a row in registers; a workgroup takes OCH_NORM_THREADS / T rows at a time,
+/* Rows of at most 8 T V elements: T threads keep a row in registers; a workgroup takes norm_rows(T) rows at a time,
    in steps of the grid, and its threads' sums for dw stay in registers until its last row. T = 64: the four waves' sums meet
-   in LDS then. */
+   in LDS then. 16384 rows of 4096 bfloat16 features with dh: 55 us (4.8 TB/s), the last step's 3 us included. */
 template <int DT, int T, int V>
-__global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_kernel(const NormGradParams p)
+__global__ __launch_bounds__(T * norm_rows(T)) void norm_grad_kernel(const NormGradParams p)
 {
    typedef typename Wide<DT>::E E;
-   constexpr int ROWS = OCH_NORM_THREADS / T;
-   __shared__ float part[OCH_NORM_THREADS / 64];
+   constexpr int ROWS = norm_rows(T);
+   __shared__ float part[T * ROWS / 64];
    __shared__ __align__(16) float meet[ROWS > 1 ? ROWS * T * V * 8 : 4];
    const int first = (int)(threadIdx.x % T) * 8, n = (int)p.n;
    float w[V][8], dw[V][8];
@@ -299,7 +316,7 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_kernel(const NormG
          for (int e = 0; e < 8; e++) s = __builtin_fmaf(a[v].get(e) * w[v][e], b[v].get(e) * rstd, s);
          sum += s;
       }
-      const float mean = group_sum<T>(sum, part) / (float)p.n;
+      const float mean = group_sum<T>(sum, part) * p.inverse;
 #pragma unroll
       for (int v = 0; v < V; v++)
       {  const int at = first + v * T * 8;
@@ -369,10 +386,13 @@ __global__ __launch_bounds__(1024) void norm_grad_finish_kernel(const float *par
    dW[at] = s;
 }
 
+/* Workgroups: each costs n floats written and read again for dw, so as few as keep the memory busy, and their row loops long.
+   2^26 values with dw: 4096 features 55.5 us with two per compute unit, 58.6 with four; 2048 features 58.0 with four, 60.4
+   with two; 8192 features (512 threads) 56.9 with one, 59.8 with two of 256 threads. */
 template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipStream_t stream)
 {
    const int rows_at_once = p.n <= 1024 ? 4 : 1;
-   uint64_t groups = 4 * (uint64_t)gemm_compute_units();
+   uint64_t groups = (p.n <= 2048 ? 4 : p.n <= 6144 ? 2 : 1) * (uint64_t)gemm_compute_units();
    if (groups > ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once) groups = ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once;
    p.partial = nullptr;
    if (dW)
@@ -383,13 +403,13 @@ template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipSt
       if (stream_gemm_workspace(stream, &ws) != 0) return -1;
       p.partial = reinterpret_cast<float *>(ws);
    }
-#define OCH_GO(T, V) hipLaunchKernelGGL((norm_grad_kernel<DT, T, V>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p)
+#define OCH_GO(T, V) hipLaunchKernelGGL((norm_grad_kernel<DT, T, V>), dim3((unsigned)groups), dim3(T * norm_rows(T)), 0, stream, p)
    if (p.n <= 512)        OCH_GO(64, 1);
    else if (p.n <= 1024)  OCH_GO(64, 2);
    else if (p.n <= 2048)  OCH_GO(256, 1);
    else if (p.n <= 4096)  OCH_GO(256, 2);
    else if (p.n <= 6144)  OCH_GO(256, 3);
-   else if (p.n <= 8192)  OCH_GO(256, 4);
+   else if (p.n <= 8192)  OCH_GO(512, 2);
    else hipLaunchKernelGGL((norm_grad_long_kernel<DT>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p);
 #undef OCH_GO
    OCH_CHECK_LAUNCH();
@@ -431,7 +451,7 @@ extern "C" int och_rms_norm(int dtype, size_t n, size_t rows, const void *X, ptr
       return set_error("rms_norm: misaligned pointer");
    NormParams p;
    p.X = (const char *)X; p.R = (const char *)R; p.W = (const char *)W; p.H = (char *)H; p.Y = (char *)Y; p.S = S; p.rstd = rstd;
-   p.ldX = ldX; p.ldR = ldR; p.ldH = ldH; p.ldY = ldY; p.ldS = ldS; p.n = (int64_t)n; p.rows = (int64_t)rows; p.eps = eps; p.w_float = (dtype_w == OCH_FLOAT);
+   p.ldX = ldX; p.ldR = ldR; p.ldH = ldH; p.ldY = ldY; p.ldS = ldS; p.n = (int64_t)n; p.rows = (int64_t)rows; p.eps = eps; p.inverse = 1.0f / (float)n; p.w_float = (dtype_w == OCH_FLOAT);
    hipStream_t s = as_stream(stream);
 #define OCH_GO(DT) (!code ? norm_launch<DT, 0>(p, s) : dtype_y == OCH_FLOAT8_E4M3 ? norm_launch<DT, OCH_FLOAT8_E4M3>(p, s) : norm_launch<DT, OCH_FLOAT8_E5M2>(p, s))
    return OCH_BY_WIDE(dtype, OCH_GO);
@@ -454,7 +474,7 @@ extern "C" int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *d
    if ((uintptr_t)dY % es || (uintptr_t)H % es || (uintptr_t)dH % es || (uintptr_t)dX % es || (uintptr_t)rstd % 4) return set_error("rms_norm_grad: misaligned pointer");
    NormGradParams p;
    p.dY = (const char *)dY; p.H = (const char *)H; p.W = (const char *)W; p.dH = (const char *)dH; p.dX = (char *)dX; p.rstd = rstd; p.partial = nullptr;
-   p.lddY = lddY; p.ldH = ldH; p.lddH = lddH; p.lddX = lddX; p.n = (int64_t)n; p.rows = (int64_t)rows; p.w_float = (dtype_w == OCH_FLOAT);
+   p.lddY = lddY; p.ldH = ldH; p.lddH = lddH; p.lddX = lddX; p.n = (int64_t)n; p.rows = (int64_t)rows; p.inverse = 1.0f / (float)n; p.w_float = (dtype_w == OCH_FLOAT);
 #define OCH_GO(DT) norm_grad_launch<DT>(p, dW, as_stream(stream))
    return OCH_BY_WIDE(dtype, OCH_GO);
 #undef OCH_GO
