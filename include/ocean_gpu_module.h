@@ -100,6 +100,24 @@ int       OcDeviceGPU_properties(OcDevice *device, void *och_device_prop_out);
    launch (och_mgs_project). Q: n x k with dense columns, v: n, r: k or NULL (receives the coefficients); same GPU, same type. */
 int       OcTensorGPU_projectColumns(OcTensor *Q, OcTensor *v, OcTensor *r);
 
+/* 8-bit floating point with block scales, beside the module table as well (och_quantize_blocks, och_rms_norm,
+   och_rms_norm_grad and och_gemm_scaled of include/ocean_hip.h, which state the formulas). Codes are UInt8 tensors whose type
+   `code` names (OCH_FLOAT8_E4M3 = 33, OCH_FLOAT8_E5M2 = 34), scales are Float tensors; the other matrices are Half or Float.
+   Matrices have dense columns; a tensor with one dimension is one column. All on the same GPU, in native byte order; results
+   are written on the stream of the first one and ordered by the read / write protocol like every other operation's.
+   Tensors that are written must not overlap others, except where the library's entry allows it.
+      quantizeBlocks    X m x n to codes Q m x n and scales S, ceil(m / blockM) x ceil(n / blockN)
+      rmsNorm           X n x rows, residual R or NULL, weights W (n) or NULL, sum H (required with R) or NULL; Y of X's type,
+                        or UInt8 with the type `code` and scales S, ceil(n / 128) x rows; rstd (rows, Float) or NULL
+      rmsNormGradient   dY, H n x rows, rstd, W or NULL, dH (gradient of the sum) or NULL; dX n x rows, dW (n, Float) or NULL
+      gemmScaled        C <- alpha op(A) op(B) + beta C; the sizes of SA and SB say whether a scale covers 1 or 128 rows of
+                        op(A) and columns of op(B) */
+int       OcTensorGPU_quantizeBlocks(OcTensor *X, int code, OcSize blockM, OcSize blockN, OcTensor *Q, OcTensor *S);
+int       OcTensorGPU_rmsNorm(OcTensor *X, OcTensor *R, OcTensor *W, double eps, int code, OcTensor *H, OcTensor *Y, OcTensor *S, OcTensor *rstd);
+int       OcTensorGPU_rmsNormGradient(OcTensor *dY, OcTensor *H, OcTensor *rstd, OcTensor *W, OcTensor *dH, OcTensor *dX, OcTensor *dW);
+int       OcTensorGPU_gemmScaled(double alpha, OcTensor *A, int codeA, char transA, OcTensor *SA, OcTensor *B, int codeB, char transB, OcTensor *SB,
+                                 double beta, OcTensor *C);
+
 #ifdef __cplusplus
 }
 #endif

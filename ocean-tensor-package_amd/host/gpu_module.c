@@ -578,6 +578,141 @@ int OcTensorGPU_projectColumns(OcTensor *Q, OcTensor *v, OcTensor *r)
    return OcTensor_finishRead(v, Q);
 }
 
+/* ---- beside the table: 8-bit floating point with block scales (no counterpart in the reference) ------------------------ */
+#define OC_F8_BLOCK 128
+#define OC_F8_BLOCKS(x) (((x) + OC_F8_BLOCK - 1) / OC_F8_BLOCK)
+/* pointer, sizes and leading dimension (in elements) of a matrix with dense columns on the given GPU; t may be NULL */
+typedef struct { OcTensor *t; char *data; OcSize m, n; OcIndex ld; } F8Matrix;
+static int f8_matrix(const char *name, const char *what, OcTensor *t, OcDevice *device, F8Matrix *r)
+{  OcIndex es;
+   memset(r, 0, sizeof(*r));
+   if ((r->t = t) == NULL) return 0;
+   if (t->device != device || !OcDeviceGPU_isInstance(device)) OcError(-1, "%s: all tensors must be on the same GPU device", name);
+   if (OcTensor_isByteswapped(t)) OcError(-1, "%s: %s must have native byte order", name, what);
+   if (t->ndims < 1 || t->ndims > 2) OcError(-1, "%s: %s must be a matrix or a vector", name, what);
+   es = OcDType_size(t->dtype);
+   r->data = OcTensor_data(t); r->m = t->size[0]; r->n = (t->ndims == 2) ? t->size[1] : 1; r->ld = (r->m > 0) ? r->m : 1;
+   if (t->nelem == 0) return 0;
+   if (r->m > 1 && t->strides[0] != es) OcError(-1, "%s: the columns of %s must be dense", name, what);
+   if (r->n > 1)
+   {  if (t->strides[1] % es != 0 || t->strides[1] < (OcIndex)(r->m * es)) OcError(-1, "%s: the columns of %s must be dense", name, what);
+      r->ld = t->strides[1] / es;
+   }
+   return 0;
+}
+static int f8_sized(const char *name, const char *what, const F8Matrix *r, OcSize m, OcSize n)
+{  if (r->t && (r->m != m || r->n != n)) OcError(-1, "%s: %s must be %td x %td (it is %td x %td)", name, what, (ptrdiff_t)m, (ptrdiff_t)n, (ptrdiff_t)r->m, (ptrdiff_t)r->n);
+   return 0;
+}
+static int f8_typed(const char *name, const char *what, const F8Matrix *r, OcDType dtype)
+{  if (r->t && r->t->dtype != dtype) OcError(-1, "%s: %s must be of type %s (it is %s)", name, what, OcDType_name(dtype), OcDType_name(r->t->dtype));
+   return 0;
+}
+static int f8_wide(const char *name, const char *what, const F8Matrix *r)
+{  if (r->t->dtype != OcDTypeHalf && r->t->dtype != OcDTypeFloat) OcError(-1, "%s: %s must be of type half or float (it is %s)", name, what, OcDType_name(r->t->dtype));
+   return 0;
+}
+/* the operation runs on the stream of `on`: wait for the others' work before, and let them wait for it afterwards */
+static int f8_start(OcTensor *on, int n, const F8Matrix *others)
+{  int i;
+   if (activate(on->device) != 0) return -1;
+   for (i = 0; i < n; i++) if (others[i].t && OcTensor_startRead(on, others[i].t) != 0) return -1;
+   return 0;
+}
+static int f8_finish(OcTensor *on, int n, const F8Matrix *others)
+{  int i;
+   if (OcTensor_update(on) != 0) return -1;
+   for (i = 0; i < n; i++) if (others[i].t && OcTensor_finishRead(on, others[i].t) != 0) return -1;
+   return 0;
+}
+
+int OcTensorGPU_quantizeBlocks(OcTensor *X, int code, OcSize blockM, OcSize blockN, OcTensor *Q, OcTensor *S)
+{  static const char *name = "quantizeBlocks";
+   F8Matrix x, q, o[2];                                              /* o: the input, the scales */
+   if (X == NULL || Q == NULL || S == NULL) OcError(-1, "%s: missing operand", name);
+   if (f8_matrix(name, "X", X, Q->device, &o[0]) != 0 || f8_matrix(name, "Q", Q, Q->device, &q) != 0 || f8_matrix(name, "S", S, Q->device, &o[1]) != 0) return -1;
+   x = o[0];
+   if (blockM < 1 || blockN < 1) OcError(-1, "%s: invalid block size", name);
+   if (f8_wide(name, "X", &x) != 0 || f8_typed(name, "Q", &q, OcDTypeUInt8) != 0 || f8_typed(name, "S", &o[1], OcDTypeFloat) != 0) return -1;
+   if (f8_sized(name, "Q", &q, x.m, x.n) != 0 || f8_sized(name, "S", &o[1], (x.m + blockM - 1) / blockM, (x.n + blockN - 1) / blockN) != 0) return -1;
+   if (f8_start(Q, 2, o) != 0) return -1;
+   OCH_CALL(och_quantize_blocks(X->dtype, code, (size_t)x.m, (size_t)x.n, x.data, x.ld, (size_t)blockM, (size_t)blockN, q.data, q.ld,
+                                (float *)o[1].data, o[1].ld, GPU_STREAM(Q)));
+   return f8_finish(Q, 2, o);
+}
+
+int OcTensorGPU_rmsNorm(OcTensor *X, OcTensor *R, OcTensor *W, double eps, int code, OcTensor *H, OcTensor *Y, OcTensor *S, OcTensor *rstd)
+{  static const char *name = "rmsNorm";
+   enum { INPUT, RESIDUAL, WEIGHTS, SUM, SCALES, RSTD, OTHERS };
+   F8Matrix o[OTHERS], y; int coded;
+   if (X == NULL || Y == NULL || (R != NULL && H == NULL)) OcError(-1, "%s: missing operand", name);
+   if (f8_matrix(name, "X", X, Y->device, &o[INPUT]) != 0 || f8_matrix(name, "R", R, Y->device, &o[RESIDUAL]) != 0 || f8_matrix(name, "W", W, Y->device, &o[WEIGHTS]) != 0 ||
+       f8_matrix(name, "H", H, Y->device, &o[SUM]) != 0 || f8_matrix(name, "S", S, Y->device, &o[SCALES]) != 0 || f8_matrix(name, "rstd", rstd, Y->device, &o[RSTD]) != 0 ||
+       f8_matrix(name, "Y", Y, Y->device, &y) != 0 || f8_wide(name, "X", &o[INPUT]) != 0) return -1;
+   coded = (Y->dtype == OcDTypeUInt8);
+   if (coded && S == NULL) OcError(-1, "%s: missing operand", name);
+   if (!coded && S != NULL) OcError(-1, "%s: an output without codes has no scales", name);
+   if (f8_typed(name, "R", &o[RESIDUAL], X->dtype) != 0 || f8_typed(name, "H", &o[SUM], X->dtype) != 0 || (!coded && f8_typed(name, "Y", &y, X->dtype) != 0) ||
+       f8_typed(name, "S", &o[SCALES], OcDTypeFloat) != 0 || f8_typed(name, "rstd", &o[RSTD], OcDTypeFloat) != 0) return -1;
+   if (W && W->dtype != OcDTypeFloat && f8_typed(name, "W", &o[WEIGHTS], X->dtype) != 0) return -1;
+   if (f8_sized(name, "R", &o[RESIDUAL], o[INPUT].m, o[INPUT].n) != 0 || f8_sized(name, "H", &o[SUM], o[INPUT].m, o[INPUT].n) != 0 ||
+       f8_sized(name, "Y", &y, o[INPUT].m, o[INPUT].n) != 0 || f8_sized(name, "W", &o[WEIGHTS], o[INPUT].m, 1) != 0 ||
+       f8_sized(name, "S", &o[SCALES], OC_F8_BLOCKS(o[INPUT].m), o[INPUT].n) != 0 || f8_sized(name, "rstd", &o[RSTD], o[INPUT].n, 1) != 0) return -1;
+   if (f8_start(Y, OTHERS, o) != 0) return -1;
+   OCH_CALL(och_rms_norm(X->dtype, (size_t)o[INPUT].m, (size_t)o[INPUT].n, o[INPUT].data, o[INPUT].ld, o[RESIDUAL].data, o[RESIDUAL].ld, o[SUM].data, o[SUM].ld,
+                         W ? (int)W->dtype : (int)X->dtype, o[WEIGHTS].data, (float)eps, coded ? code : (int)X->dtype, y.data, y.ld,
+                         (float *)o[SCALES].data, o[SCALES].ld, (float *)o[RSTD].data, GPU_STREAM(Y)));
+   return f8_finish(Y, OTHERS, o);
+}
+
+int OcTensorGPU_rmsNormGradient(OcTensor *dY, OcTensor *H, OcTensor *rstd, OcTensor *W, OcTensor *dH, OcTensor *dX, OcTensor *dW)
+{  static const char *name = "rmsNormGradient";
+   enum { OUTPUT, SUM, RSTD, WEIGHTS, DSUM, DWEIGHTS, OTHERS };
+   F8Matrix o[OTHERS], x;
+   if (dY == NULL || H == NULL || rstd == NULL || dX == NULL) OcError(-1, "%s: missing operand", name);
+   if (f8_matrix(name, "dY", dY, dX->device, &o[OUTPUT]) != 0 || f8_matrix(name, "H", H, dX->device, &o[SUM]) != 0 || f8_matrix(name, "rstd", rstd, dX->device, &o[RSTD]) != 0 ||
+       f8_matrix(name, "W", W, dX->device, &o[WEIGHTS]) != 0 || f8_matrix(name, "dH", dH, dX->device, &o[DSUM]) != 0 || f8_matrix(name, "dW", dW, dX->device, &o[DWEIGHTS]) != 0 ||
+       f8_matrix(name, "dX", dX, dX->device, &x) != 0 || f8_wide(name, "dX", &x) != 0) return -1;
+   if (f8_typed(name, "dY", &o[OUTPUT], dX->dtype) != 0 || f8_typed(name, "H", &o[SUM], dX->dtype) != 0 || f8_typed(name, "dH", &o[DSUM], dX->dtype) != 0 ||
+       f8_typed(name, "rstd", &o[RSTD], OcDTypeFloat) != 0 || f8_typed(name, "dW", &o[DWEIGHTS], OcDTypeFloat) != 0) return -1;
+   if (W && W->dtype != OcDTypeFloat && f8_typed(name, "W", &o[WEIGHTS], dX->dtype) != 0) return -1;
+   if (f8_sized(name, "dY", &o[OUTPUT], x.m, x.n) != 0 || f8_sized(name, "H", &o[SUM], x.m, x.n) != 0 || f8_sized(name, "dH", &o[DSUM], x.m, x.n) != 0 ||
+       f8_sized(name, "rstd", &o[RSTD], x.n, 1) != 0 || f8_sized(name, "W", &o[WEIGHTS], x.m, 1) != 0 || f8_sized(name, "dW", &o[DWEIGHTS], x.m, 1) != 0) return -1;
+   if (f8_start(dX, OTHERS, o) != 0) return -1;
+   OCH_CALL(och_rms_norm_grad(dX->dtype, (size_t)x.m, (size_t)x.n, o[OUTPUT].data, o[OUTPUT].ld, o[SUM].data, o[SUM].ld, (const float *)o[RSTD].data,
+                              W ? (int)W->dtype : (int)dX->dtype, o[WEIGHTS].data, o[DSUM].data, o[DSUM].ld, x.data, x.ld, (float *)o[DWEIGHTS].data, GPU_STREAM(dX)));
+   return f8_finish(dX, OTHERS, o);
+}
+
+/* rows of the scales' matrix (columns when it is transposed) of an operand with `outer` rows of op(A): one scale each or one
+   per 128; 0: neither */
+static int f8_outer_block(OcSize scales, OcSize outer)
+{  if (scales == OC_F8_BLOCKS(outer)) return OC_F8_BLOCK;
+   return scales == outer ? 1 : 0;
+}
+int OcTensorGPU_gemmScaled(double alpha, OcTensor *A, int codeA, char transA, OcTensor *SA, OcTensor *B, int codeB, char transB, OcTensor *SB, double beta, OcTensor *C)
+{  static const char *name = "gemmScaled";
+   enum { LEFT, LEFT_SCALES, RIGHT, RIGHT_SCALES, OTHERS };
+   F8Matrix o[OTHERS], c; OcSize M, N, K; int ta = (transA == 'T' || transA == 't'), tb = (transB == 'T' || transB == 't'), blockA, blockB;
+   if (A == NULL || SA == NULL || B == NULL || SB == NULL || C == NULL) OcError(-1, "%s: missing operand", name);
+   if (f8_matrix(name, "A", A, C->device, &o[LEFT]) != 0 || f8_matrix(name, "SA", SA, C->device, &o[LEFT_SCALES]) != 0 || f8_matrix(name, "B", B, C->device, &o[RIGHT]) != 0 ||
+       f8_matrix(name, "SB", SB, C->device, &o[RIGHT_SCALES]) != 0 || f8_matrix(name, "C", C, C->device, &c) != 0 || f8_wide(name, "C", &c) != 0) return -1;
+   if ((!ta && transA != 'N' && transA != 'n') || (!tb && transB != 'N' && transB != 'n')) OcError(-1, "%s: transA and transB are 'N' or 'T'", name);
+   if (f8_typed(name, "A", &o[LEFT], OcDTypeUInt8) != 0 || f8_typed(name, "B", &o[RIGHT], OcDTypeUInt8) != 0 ||
+       f8_typed(name, "SA", &o[LEFT_SCALES], OcDTypeFloat) != 0 || f8_typed(name, "SB", &o[RIGHT_SCALES], OcDTypeFloat) != 0) return -1;
+   M = ta ? o[LEFT].n : o[LEFT].m; K = ta ? o[LEFT].m : o[LEFT].n; N = tb ? o[RIGHT].m : o[RIGHT].n;
+   if (K != (tb ? o[RIGHT].n : o[RIGHT].m) || c.m != M || c.n != N) OcError(-1, "%s: mismatch in tensor sizes", name);
+   blockA = f8_outer_block(ta ? o[LEFT_SCALES].n : o[LEFT_SCALES].m, M);
+   blockB = f8_outer_block(tb ? o[RIGHT_SCALES].m : o[RIGHT_SCALES].n, N);
+   if (blockA == 0 || blockB == 0 || (ta ? o[LEFT_SCALES].m : o[LEFT_SCALES].n) != OC_F8_BLOCKS(K) || (tb ? o[RIGHT_SCALES].n : o[RIGHT_SCALES].m) != OC_F8_BLOCKS(K))
+      OcError(-1, "%s: the scales do not fit their matrices", name);
+   if (f8_start(C, OTHERS, o) != 0) return -1;
+   OCH_CALL(och_gemm_scaled(codeA, codeB, C->dtype, ta ? 'T' : 'N', tb ? 'T' : 'N', (size_t)M, (size_t)N, (size_t)K, (float)alpha,
+                            o[LEFT].data, o[LEFT].ld, (const float *)o[LEFT_SCALES].data, o[LEFT_SCALES].ld, (size_t)blockA,
+                            o[RIGHT].data, o[RIGHT].ld, (const float *)o[RIGHT_SCALES].data, o[RIGHT_SCALES].ld, (size_t)blockB, (float)beta, c.data, c.ld, GPU_STREAM(C)));
+   return f8_finish(C, OTHERS, o);
+}
+
 /* ---- module table and registration (module_core_gpu.c:40-145) ------------------------------------ */
 static int initializeContext(OcDevice *device, OcDeviceModule *deviceModule, void **context)
 {  OcModuleCoreGPU_Context *ctx;

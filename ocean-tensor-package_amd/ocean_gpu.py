@@ -11,6 +11,7 @@ A device is callable on a numpy array, as `ocean.gpu[0](tensor)` is: the data mo
 result is a tensor of the host layer (ocean_host), which `ocean_host.to_numpy` brings back.
 """
 import builtins as _py
+import collections as _collections
 import ctypes as C
 
 import ocean_hip as _hip
@@ -833,6 +834,83 @@ def gemm(alpha, a, b, beta=None, c=None, transA="N", transB="N"):
     dst = _host.TP() if c is None else c._h
     _host.check(_host.lib.OcTensor_gemmTensors(al._h, a._h, transA.encode(), b._h, transB.encode(), be._h if be is not None else None, C.byref(dst)))
     return c if c is not None else tensor(dst)
+
+
+# ---- 8-bit floating point with block scales (no counterpart in the reference): codes are uint8 tensors, their type is named
+# "e4m3" or "e5m2"; scales are float tensors, one per block of 128 ----
+_CODES = {"e4m3": _hip.FLOAT8_E4M3, "e5m2": _hip.FLOAT8_E5M2}
+RMSNorm = _collections.namedtuple("RMSNorm", "y scales sum rstd")
+RMSNorm.__doc__ = "What rmsNorm returns; scales and sum are None where there are none."
+
+
+def _code(name):
+    if name not in _CODES:
+        raise ValueError("the code type is 'e4m3' or 'e5m2' (got %r)" % (name,))
+    return _CODES[name]
+
+
+def _like(t, dt=None, size=None):
+    """A new tensor on t's device, with dense columns."""
+    return tensor(t.size if size is None else size, t.dtype if dt is None else dt, t.device)
+
+
+def _blocks(t, bm, bn):
+    if t.ndims < 1:
+        raise ValueError("the operand is a matrix or a vector")
+    n = _columns(t)
+    return (-(-t.size[0] // bm), -(-n // bn)) if t.ndims > 1 else (-(-t.size[0] // bm),)
+
+
+def _columns(t):
+    return t.size[1] if t.ndims > 1 else 1
+
+
+def _handle(t):
+    return None if t is None else t._h
+
+
+def quantizeBlocks(x, block=(128, 1), code="e4m3"):
+    """The half or float matrix x as 8-bit codes of the same size and the scales of its blocks of 128 x 1, 1 x 128 or
+    128 x 128 elements: (codes, scales)."""
+    if len(block) != 2 or _py.min(block) < 1:
+        raise ValueError("quantizeBlocks: blocks are 128 x 1, 1 x 128 or 128 x 128")
+    q, s = _like(x, uint8), _like(x, float, _blocks(x, *block))
+    _host.check(_host.lib.OcTensorGPU_quantizeBlocks(x._h, _code(code), block[0], block[1], q._h, s._h))
+    return q, s
+
+
+def rmsNorm(x, weight=None, eps=1e-5, residual=None, code=None):
+    """Root-mean-square norm of the columns of x (features x tokens, half or float), of x + residual when that is given:
+    an RMSNorm of the output y, the scales of its blocks of 128 features when `code` asks for an 8-bit output, the sum when
+    there is a residual, and the reciprocal roots that the gradient needs."""
+    y = _like(x, uint8 if code is not None else None)
+    s = _like(x, float, _blocks(x, 128, 1)) if code is not None else None
+    h = _like(x) if residual is not None else None
+    rstd = _like(x, float, (_columns(x),))
+    _host.check(_host.lib.OcTensorGPU_rmsNorm(x._h, _handle(residual), _handle(weight), eps, _code(code) if code is not None else 0, _handle(h), y._h, _handle(s),
+                                              rstd._h))
+    return RMSNorm(y, s, h, rstd)
+
+
+def rmsNormGradient(dy, h, rstd, weight=None, dsum=None):
+    """Gradients of rmsNorm: (dx, dw) from the gradient dy of its output, h = what was normalised (x, or the sum), the
+    reciprocal roots, and the gradient dsum that reaches the sum beside the output. dx is that of x and of the residual."""
+    dx, dw = _like(h), _like(h, float, (h.size[0],))
+    _host.check(_host.lib.OcTensorGPU_rmsNormGradient(dy._h, h._h, rstd._h, _handle(weight), _handle(dsum), dx._h, dw._h))
+    return dx, dw
+
+
+def gemmScaled(alpha, a, sa, b, sb, beta=0.0, c=None, transA="N", transB="N", codeA="e4m3", codeB="e4m3", dt=float):
+    """alpha op(A) op(B) + beta C of two matrices in 8-bit codes with their scales, as quantizeBlocks and rmsNorm make them;
+    C is written if given, or a new matrix of type dt (half or float)."""
+    if c is None:
+        if beta != 0:
+            raise ValueError("gemmScaled: beta without C")
+        if a.ndims < 1 or b.ndims < 1:
+            raise ValueError("gemmScaled: the operands are matrices")
+        c = _like(a, dt, (_columns(a) if transA in "Tt" else a.size[0], b.size[0] if transB in "Tt" else _columns(b)))
+    _host.check(_host.lib.OcTensorGPU_gemmScaled(alpha, a._h, _code(codeA), transA.encode(), sa._h, b._h, _code(codeB), transB.encode(), sb._h, beta, c._h))
+    return c
 
 
 def _device_call(self, array, dt=None):

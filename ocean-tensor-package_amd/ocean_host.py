@@ -125,6 +125,10 @@ lib.OcTensor_maskedFill.argtypes = [TP, TP, C.POINTER(Scalar)]
 lib.OcTensor_stepsInt64.argtypes = [TP, C.c_int64, C.c_int64]
 lib.OcTensor_stepsDouble.argtypes = [TP, C.c_double, C.c_double]
 lib.OcTensorGPU_projectColumns.argtypes = [TP, TP, TP]
+lib.OcTensorGPU_quantizeBlocks.argtypes = [TP, C.c_int, C.c_ssize_t, C.c_ssize_t, TP, TP]
+lib.OcTensorGPU_rmsNorm.argtypes = [TP, TP, TP, C.c_double, C.c_int, TP, TP, TP, TP]
+lib.OcTensorGPU_rmsNormGradient.argtypes = [TP, TP, TP, TP, TP, TP, TP]
+lib.OcTensorGPU_gemmScaled.argtypes = [C.c_double, TP, C.c_int, C.c_char, TP, TP, C.c_int, C.c_char, TP, C.c_double, TP]
 lib.OcTensor_find.restype = TP
 lib.OcTensor_find.argtypes = [TP]
 lib.OcTensor_maskToOffset.restype = TP
