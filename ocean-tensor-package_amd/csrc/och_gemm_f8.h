@@ -122,6 +122,12 @@ template <bool KC, int R> __device__ __forceinline__ och_i32x8 f8_fragment(const
    return f;
 }
 
+/* one float per lane from memory to LDS, as load_to_lds moves sixteen bytes */
+static __device__ __forceinline__ void load_float_to_lds(const char *base, uint32_t offset, uint32_t target)
+{
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(target), "v"(offset), "s"(base) : "memory");
+}
+
 /* one element of C: s is the finished sum */
 template <int DT> __device__ __forceinline__ void f8_finish(char *C, int64_t at, float s, float alpha, float beta)
 {  typedef typename Wide<DT>::E E;

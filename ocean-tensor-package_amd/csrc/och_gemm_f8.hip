@@ -97,7 +97,7 @@ extern "C" int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, 
    const bool e5a = dtypeA == OCH_FLOAT8_E5M2, e5b = dtypeB == OCH_FLOAT8_E5M2;
    hipStream_t s = as_stream(stream);
    /* few columns on their own kernel, which loads 16 bytes at a time and counts bytes within its rows in 32 bits */
-   const bool aligned = (((uintptr_t)A | (uintptr_t)B | (uintptr_t)ldA | (uintptr_t)ldB) & 15) == 0, near = ldA < (1 << 25) && ldB < (1 << 25);
+   const bool aligned = (((uintptr_t)A | (uintptr_t)B | (uintptr_t)ldA | (uintptr_t)ldB) & 15) == 0, near = ldA < (1 << 25) && ldB < (1 << 25) && ldSA < (1 << 24) && ldSB < (1 << 24);
    if (N <= 64 && akc && bkc && aligned && near)
       return e5a ? (e5b ? gemm_f8_few_55(p, s) : gemm_f8_few_54(p, s)) : (e5b ? gemm_f8_few_45(p, s) : gemm_f8_few_44(p, s));
    /* float results need the wide sums, and chunks of 16 rows must not pass the end of an operand that is contiguous along them */

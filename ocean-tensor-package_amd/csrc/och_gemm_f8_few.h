@@ -3,28 +3,32 @@
  * columns may be idle, are nearly free.
  *
  * A workgroup owns 16 TM rows of A and all columns; its W waves share out the slabs of 128 k (wave w takes slabs w, w + W,
- * ..., beginning at another one in every workgroup), so that a few thousand waves are in flight whatever M is. Every wave
+ * ...), so that a few thousand waves are in flight whatever M is. The workgroups of a die (every eighth) begin at different
+ * slabs, or else they would all read the same k of rows that lie a power of two apart, which one channel of the die's cache
+ * serves: 8192 x 16 x 8192 14.8 us instead of 19.2. Every wave
  * has a slot of its own in LDS that loads from memory fill directly, eight rows of 128 consecutive bytes per load: with
  * fragments loaded straight into registers a load covers sixteen rows of 64 bytes, which the first-level cache serves at
  * 15 instead of 38 bytes a cycle. No wave waits for another before the end, where the waves' sums meet in LDS and are added
- * in the order of the waves. Two tiles of rows share the columns' codes where there are more than 16 columns: these come
- * from the second-level cache once per workgroup and slab.
+ * in the order of the waves. Two tiles of rows share the columns' codes where there are more than 16 columns and rows enough:
+ * these come from the second-level cache once per workgroup and slab.
  *
- * Measured: 14336 x 1 x 4096 11.6 us, 8192 x 16 x 8192 15 us, 8192 x 48 x 8192 20 us (on 128 x 128 tiles 16, 22 and 22). */
+ * Measured, operands of 200 MB in turn: 14336 x 1 x 4096 10.9 us (5.4 TB/s), 8192 x 16 x 8192 11.7 us (5.8 TB/s), 8192 x 48
+ * x 8192 14.9 us (4.6 TB/s); every 16 columns more cost 3 us, their codes being read by all 256 workgroups (11 TB/s from the second-level
+ * cache). Two slots per wave, the next but one slab under way, change nothing at these sizes. On 128 x 128 tiles 16, 22, 22. */
 #pragma once
 #include "och_gemm_f8_tile.h"
 #pragma clang diagnostic ignored "-Winline-asm"
 
 namespace och {
 
-static constexpr uint32_t f8_few_waves(int TM) { return TM == 1 ? 16 : 8; }      /* at most, per workgroup: two tiles of rows need over 128 registers */
-static constexpr uint32_t f8_few_slot(int TM, int TN) { return (uint32_t)(TM + TN) * 16 * OCH_F8_SLAB; }
+static constexpr uint32_t f8_few_waves(int TN) { return TN == 1 ? 16 : 8; }      /* at most, per workgroup: more than 16 columns need over 128 registers */
+static constexpr uint32_t f8_few_slot(int TM, int TN) { return (uint32_t)(TM + TN) * 16 * OCH_F8_SLAB + 512; }      /* codes, 64 scales of A, 64 of B */
 
-template <bool E5A, bool E5B, bool WIDE, bool ROWS, int TM, int TN>
-__global__ __launch_bounds__(64 * f8_few_waves(TM)) void gemm_f8_few_kernel(const F8GemmParams p)
+template <bool E5A, bool E5B, bool WIDE, int TM, int TN>
+__global__ __launch_bounds__(64 * f8_few_waves(TN)) void gemm_f8_few_kernel(const F8GemmParams p)
 {
    typedef F8Slab<true, 32> L;
-   constexpr uint32_t SLOT = f8_few_slot(TM, TN), SLOT_B = TM * 16 * OCH_F8_SLAB;
+   constexpr uint32_t SLOT = f8_few_slot(TM, TN), SLOT_B = TM * 16 * OCH_F8_SLAB, SLOT_SCALES = SLOT - 512;
    extern __shared__ __align__(16) char lds_few[];
    const uint32_t lane = threadIdx.x & 63, g = lane / 16, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x / 64;
    const uint32_t m0 = blockIdx.x * 16 * TM;
@@ -48,48 +52,32 @@ __global__ __launch_bounds__(64 * f8_few_waves(TM)) void gemm_f8_few_kernel(cons
    {  const uint32_t r = row0 + 8 * e, last = p.N - 1;
       ob[e] = (r < last ? r : last) * (uint32_t)p.ldB + k0;
    }
-   const float *sa[TM][4], *sb[TN];
+   /* lane l brings the scales of row l and of column l */
+   const uint32_t last_row = p.M - 1 - m0 < 16 * TM - 1 ? p.M - 1 - m0 : 16 * TM - 1, last_column = p.N - 1 < 16 * TN - 1 ? p.N - 1 : 16 * TN - 1;
+   const uint32_t osa = (((m0 + (lane < last_row ? lane : last_row)) >> p.shiftA) - (m0 >> p.shiftA)) * (uint32_t)p.sa_m * 4;
+   const uint32_t osb = ((lane < last_column ? lane : last_column) >> p.shiftB) * (uint32_t)p.sb_n * 4;
+   const char *scalesA = (const char *)(p.SA + (int64_t)(m0 >> p.shiftA) * p.sa_m), *scalesB = (const char *)p.SB;
 #pragma unroll
    for (int i = 0; i < TM; i++)
-   {
-#pragma unroll
-      for (int r = 0; r < (ROWS ? 4 : 1); r++)
-      {  const uint32_t q = ROWS ? m0 + 16 * i + 4 * g + r : m0;
-         sa[i][r] = p.SA + (int64_t)((q < p.M ? q : p.M - 1) >> p.shiftA) * p.sa_m;
-      }
 #pragma unroll
       for (int j = 0; j < TN; j++) acc[i][j] = zero;
-   }
-#pragma unroll
-   for (int j = 0; j < TN; j++)
-   {  const uint32_t n = 16 * j + lane % 16, c = n < p.N ? n : p.N - 1;
-      sb[j] = p.SB + (int64_t)(c >> p.shiftB) * p.sb_n;
-   }
-   och_f32x4v rs[TM]; float t[TN];                 /* scales of the slab in the slot */
-   auto scales = [&](uint32_t s)
-   {
-#pragma unroll
-      for (int i = 0; i < TM; i++)
-#pragma unroll
-         for (int r = 0; r < 4; r++) rs[i][r] = sa[i][ROWS ? r : 0][(int64_t)s * p.sa_k];
-#pragma unroll
-      for (int j = 0; j < TN; j++) t[j] = sb[j][(int64_t)s * p.sb_k];
-   };
    auto fetch = [&](uint32_t s)
    {
 #pragma unroll
       for (int e = 0; e < 2 * TM; e++) load_to_lds(rowsA + (uint64_t)s * OCH_F8_SLAB, oa[e], target + 1024 * e);
 #pragma unroll
       for (int e = 0; e < 2 * TN; e++) load_to_lds(rowsB + (uint64_t)s * OCH_F8_SLAB, ob[e], target + SLOT_B + 1024 * e);
-      scales(s);
+      load_float_to_lds(scalesA + (int64_t)s * p.sa_k * 4, osa, target + SLOT_SCALES);
+      load_float_to_lds(scalesB + (int64_t)s * p.sb_k * 4, osb, target + SLOT_SCALES + 256);
    };
    /* the slot's slab: fragments to registers, then (the slot is free) `next`, then the product */
    auto use = [&](auto next)
    {  och_i32x8 ca[TM], cb[TN]; och_f32x4v r0[TM]; float t0[TN];
+      const float *rs = reinterpret_cast<const float *>(slot + SLOT_SCALES), *t = rs + 64;
 #pragma unroll
-      for (int i = 0; i < TM; i++) { ca[i] = f8_fragment<true, 32>(slot, 16 * i); r0[i] = rs[i]; }
+      for (int i = 0; i < TM; i++) { ca[i] = f8_fragment<true, 32>(slot, 16 * i); r0[i] = *reinterpret_cast<const och_f32x4v *>(rs + 16 * i + 4 * g); }
 #pragma unroll
-      for (int j = 0; j < TN; j++) { cb[j] = f8_fragment<true, 32>(slot + SLOT_B, 16 * j); t0[j] = t[j]; }
+      for (int j = 0; j < TN; j++) { cb[j] = f8_fragment<true, 32>(slot + SLOT_B, 16 * j); t0[j] = t[16 * j + lane % 16]; }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       next();
       F8Operand<WIDE> fb[TN];
@@ -108,7 +96,7 @@ __global__ __launch_bounds__(64 * f8_few_waves(TM)) void gemm_f8_few_kernel(cons
       }
    };
    const uint32_t whole = p.K / OCH_F8_SLAB, turns = wave < whole ? (whole - wave + W - 1) / W : 0;
-   uint32_t turn = turns ? blockIdx.x % turns : 0;
+   uint32_t turn = turns ? blockIdx.x / 8 % turns : 0;
    if (turns) fetch(wave + turn * W);
    for (uint32_t i = 0; i < turns; i++)
    {  turn = turn + 1 < turns ? turn + 1 : 0;
@@ -124,7 +112,9 @@ __global__ __launch_bounds__(64 * f8_few_waves(TM)) void gemm_f8_few_kernel(cons
 #pragma unroll
       for (int e = 0; e < 2 * TN; e++)
          *reinterpret_cast<och_u32x4 *>(slot + SLOT_B + 1024 * e + 16 * lane) = f8_border_chunk((const uint8_t *)rowsB + (uint64_t)whole * OCH_F8_SLAB + ob[e], valid, p.K);
-      scales(whole);
+      float *rest = reinterpret_cast<float *>(slot + SLOT_SCALES);
+      rest[lane] = *reinterpret_cast<const float *>(scalesA + (int64_t)whole * p.sa_k * 4 + osa);
+      rest[64 + lane] = *reinterpret_cast<const float *>(scalesB + (int64_t)whole * p.sb_k * 4 + osb);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       use([]() { });
    }
@@ -150,31 +140,33 @@ __global__ __launch_bounds__(64 * f8_few_waves(TM)) void gemm_f8_few_kernel(cons
    }
 }
 
-template <bool E5A, bool E5B, bool WIDE, bool ROWS, int TM, int TN> static int gemm_f8_few_launch(const F8GemmParams &p, hipStream_t stream)
+template <bool E5A, bool E5B, bool WIDE, int TM, int TN> static int gemm_f8_few_launch(const F8GemmParams &p, hipStream_t stream)
 {
-   auto kernel = gemm_f8_few_kernel<E5A, E5B, WIDE, ROWS, TM, TN>;
-   /* waves per workgroup: about sixteen per compute unit, no more than slabs or than their slots fit into 160 KB */
+   auto kernel = gemm_f8_few_kernel<E5A, E5B, WIDE, TM, TN>;
+   /* waves per workgroup: eight per compute unit over all, no more than slabs or than their slots fit into 160 KB */
    const uint32_t slabs = (uint32_t)(((uint64_t)p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB), groups = (p.M + 16 * TM - 1) / (16 * TM);
-   uint32_t waves = 1;
-   while (waves < f8_few_waves(TM) && waves * 2 <= slabs && 2 * waves * f8_few_slot(TM, TN) <= 163840 && (uint64_t)groups * waves < 8ull * gemm_compute_units()) waves *= 2;
+   uint32_t waves = (uint32_t)((8ull * gemm_compute_units() + groups - 1) / groups);
+   if (waves > f8_few_waves(TN)) waves = f8_few_waves(TN);
+   if (waves > slabs) waves = slabs > 0 ? slabs : 1;
+   if (waves > 163840 / f8_few_slot(TM, TN)) waves = 163840 / f8_few_slot(TM, TN);
    const size_t lds = (size_t)waves * f8_few_slot(TM, TN);
    if (lds > 65536) OCH_CHECK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
    hipLaunchKernelGGL(kernel, dim3(groups), dim3(64 * waves), lds, stream, p);
    OCH_CHECK_LAUNCH();
    return 0;
 }
-template <bool E5A, bool E5B, bool WIDE, bool ROWS> static int gemm_f8_few_columns(const F8GemmParams &p, hipStream_t stream)
+template <bool E5A, bool E5B, bool WIDE> static int gemm_f8_few_columns(const F8GemmParams &p, hipStream_t stream)
 {
-   if (p.N <= 16) return gemm_f8_few_launch<E5A, E5B, WIDE, ROWS, 1, 1>(p, stream);
-   if (p.N <= 32) return gemm_f8_few_launch<E5A, E5B, WIDE, ROWS, 2, 2>(p, stream);
-   if (p.N <= 48) return gemm_f8_few_launch<E5A, E5B, WIDE, ROWS, 2, 3>(p, stream);
-   return gemm_f8_few_launch<E5A, E5B, WIDE, ROWS, 2, 4>(p, stream);
+   if (p.N <= 16) return gemm_f8_few_launch<E5A, E5B, WIDE, 1, 1>(p, stream);
+   /* single tiles of rows where pairs would leave compute units idle: 4096 x 32 x 14336 12.9 us against 16.2 */
+   const bool single = p.M <= 16u * (uint32_t)gemm_compute_units();
+   if (p.N <= 32) return single ? gemm_f8_few_launch<E5A, E5B, WIDE, 1, 2>(p, stream) : gemm_f8_few_launch<E5A, E5B, WIDE, 2, 2>(p, stream);
+   if (p.N <= 48) return single ? gemm_f8_few_launch<E5A, E5B, WIDE, 1, 3>(p, stream) : gemm_f8_few_launch<E5A, E5B, WIDE, 2, 3>(p, stream);
+   return single ? gemm_f8_few_launch<E5A, E5B, WIDE, 1, 4>(p, stream) : gemm_f8_few_launch<E5A, E5B, WIDE, 2, 4>(p, stream);
 }
 template <bool E5A, bool E5B> static int gemm_f8_few(const F8GemmParams &p, hipStream_t stream)
 {
-   const bool wide = p.dtypeC == OCH_FLOAT, rows = p.shiftA == 0;
-   return wide ? (rows ? gemm_f8_few_columns<E5A, E5B, true, true>(p, stream) : gemm_f8_few_columns<E5A, E5B, true, false>(p, stream))
-               : (rows ? gemm_f8_few_columns<E5A, E5B, false, true>(p, stream) : gemm_f8_few_columns<E5A, E5B, false, false>(p, stream));
+   return p.dtypeC == OCH_FLOAT ? gemm_f8_few_columns<E5A, E5B, true>(p, stream) : gemm_f8_few_columns<E5A, E5B, false>(p, stream);
 }
 
 } /* namespace och */

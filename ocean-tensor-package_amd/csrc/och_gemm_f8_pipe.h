@@ -24,12 +24,6 @@ namespace och {
 #define OCH_F8_PIPE 256
 #define OCH_F8_PIPE_THREADS 512
 
-/* one float per lane from memory to LDS, as load_to_lds moves sixteen bytes */
-static __device__ __forceinline__ void load_float_to_lds(const char *base, uint32_t offset, uint32_t target)
-{
-   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(target), "v"(offset), "s"(base) : "memory");
-}
-
 /* The four loads of a slab's 256 rows that a wave issues, 1 KB each: chunks 64 (4 wave + e) + lane. Rows that do not exist
    repeat the last (KC) or the last sixteen (!KC: the number of rows is a multiple of 16 there). */
 template <bool KC> struct F8PipeLoads
