@@ -448,7 +448,7 @@ int och_rms_norm(int dtype, size_t n, size_t rows, const void *X, ptrdiff_t ldX,
 /* be NULL); all matrices of type dtype. With u = h * rstd and g = dy * w:                                                 */
 /*    dX = rstd * (g - u * mean(g * u)) + dh,   which is the gradient of x and of r;     dW = sum over the rows of dy * u  */
 /* dX may be dY or dH itself. dW (n floats, overwritten) may be NULL; it is summed in a fixed order that depends on the    */
-/* sizes alone, through the stream's workspace: n is at most 2^24 then.                                                    */
+/* sizes and the device alone, through the stream's workspace: n is at most 2^24 then.                                     */
 int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *dY, ptrdiff_t lddY, const void *H, ptrdiff_t ldH, const float *rstd,
                       int dtype_w, const void *W, const void *dH, ptrdiff_t lddH, void *dX, ptrdiff_t lddX, float *dW, och_stream stream);
 

@@ -141,6 +141,8 @@ __device__ __forceinline__ void store_codes(uint8_t *at, och_u32x2 q, int64_t va
    }
 }
 
+/* host: a launch has fewer than 2^32 threads; more work than that goes out in pieces of this many workgroups of `threads` */
+static constexpr uint64_t most_groups(uint64_t threads) { return 0xFFFFFFFFull / threads; }
 /* host: types that the three operations take */
 static inline bool wide_type(int dtype) { return dtype == OCH_HALF || dtype == OCH_BFLOAT16 || dtype == OCH_FLOAT; }
 static inline bool code_type(int dtype) { return dtype == OCH_FLOAT8_E4M3 || dtype == OCH_FLOAT8_E5M2; }

@@ -27,7 +27,7 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
 {
    p.tiles_m = (p.M + OCH_F8_TILE - 1) / OCH_F8_TILE; p.tiles_n = (p.N + OCH_F8_TILE - 1) / OCH_F8_TILE;
    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n, slabs = ((uint64_t)p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB, units = (uint64_t)gemm_compute_units();
-   if (tiles > 0x7FFFFFFFull) return set_error("gemm_scaled: too many tiles");
+   if (tiles > most_groups(OCH_F8_TILE_THREADS)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
    uint64_t shares = tiles * 2 <= units ? 2 * units / tiles : 1;
    if (shares > slabs / 4) shares = slabs / 4;
    const uint64_t fit = OCH_GEMM_WORKSPACE / ((uint64_t)p.M * p.N * sizeof(float));
@@ -103,7 +103,7 @@ extern "C" int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, 
    /* float results need the wide sums, and chunks of 16 rows must not pass the end of an operand that is contiguous along them */
    if (dtypeC != OCH_FLOAT && aligned && ldA < (1 << 24) && ldB < (1 << 24) && ldSA < (1 << 22) && ldSB < (1 << 22) && (akc || M % 16 == 0) && (bkc || N % 16 == 0) && gemm_f8_large(M, N))
    {  p.tiles_m = (p.M + 255) / 256; p.tiles_n = (p.N + 255) / 256;
-      if ((uint64_t)p.tiles_m * p.tiles_n > 0x7FFFFFFFull) return set_error("gemm_scaled: too many tiles");
+      if ((uint64_t)p.tiles_m * p.tiles_n > most_groups(512)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
       return e5a ? (e5b ? gemm_f8_pipe_55(p, akc, bkc, s) : gemm_f8_pipe_54(p, akc, bkc, s)) : (e5b ? gemm_f8_pipe_45(p, akc, bkc, s) : gemm_f8_pipe_44(p, akc, bkc, s));
    }
    return gemm_f8_tiles(p, e5a, e5b, akc, bkc, s);

@@ -149,6 +149,7 @@ template <bool E5A, bool E5B, bool WIDE, int TM, int TN> static int gemm_f8_few_
    if (waves > f8_few_waves(TN)) waves = f8_few_waves(TN);
    if (waves > slabs) waves = slabs > 0 ? slabs : 1;
    if (waves > 163840 / f8_few_slot(TM, TN)) waves = 163840 / f8_few_slot(TM, TN);
+   if (groups > most_groups(64 * waves)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
    const size_t lds = (size_t)waves * f8_few_slot(TM, TN);
    if (lds > 65536) OCH_CHECK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
    hipLaunchKernelGGL(kernel, dim3(groups), dim3(64 * waves), lds, stream, p);

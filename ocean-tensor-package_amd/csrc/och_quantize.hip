@@ -16,7 +16,7 @@ struct QuantizeParams
    int64_t  ldX, ldQ, ldS;              /* in elements */
    int64_t  M, N;
    uint32_t bm;                         /* blocks along M: ceil(M / 128) */
-   uint64_t blocks;
+   uint64_t blocks, first;              /* blocks of 128 x 1; workgroup 0's place in the whole */
 };
 
 /* Blocks of 128 x 1: sixteen lanes own a block, eight elements each, and take OCH_QUANTIZE_VECTORS blocks, sixteen apart,
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
    uint32_t kb[V];
 #pragma unroll
    for (int v = 0; v < V; v++)
-   {  const uint64_t b = ((uint64_t)blockIdx.x * V + v) * 16 + threadIdx.x / 16;
+   {  const uint64_t b = ((p.first + blockIdx.x) * V + v) * 16 + threadIdx.x / 16;
       const bool live = b < p.blocks;
       if (p.blocks >> 32 == 0) j[v] = (uint32_t)b / p.bm;
       else                     j[v] = (int64_t)(b / p.bm);
@@ -70,8 +70,8 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams
    typedef typename Wide<DT>::E E;
    constexpr int WORDS = Wide8<DT>::WORDS * 4, PER = 8 / WORDS;    /* of a thread; elements in a word */
    __shared__ och_u32x4 part[4][16][WORDS / 4];
-   const uint32_t kb = blockIdx.x % p.bm;
-   const int64_t nb = blockIdx.x / p.bm;
+   const uint32_t tile = (uint32_t)p.first + blockIdx.x, kb = tile % p.bm;
+   const int64_t nb = tile / p.bm;
    const int ti = threadIdx.x % 16, tj = threadIdx.x / 16;
    const int64_t i = (int64_t)kb * OCH_F8_BLOCK + ti * 8, j0 = nb * OCH_F8_BLOCK + tj, valid = p.M - i;
    Wide8<DT> v[8];
@@ -130,15 +130,18 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams
 }
 
 template <int DT, int CODE>
-static int quantize_launch(const QuantizeParams &p, bool rows, bool whole, hipStream_t stream)
+static int quantize_launch(QuantizeParams p, bool rows, bool whole, hipStream_t stream)
 {
    const uint64_t groups = rows ? (p.blocks + 16 * OCH_QUANTIZE_VECTORS - 1) / (16 * OCH_QUANTIZE_VECTORS) : (uint64_t)p.bm * ((p.N + OCH_F8_BLOCK - 1) / OCH_F8_BLOCK);
-   if (groups > 0x7FFFFFFFull) return set_error("quantize_blocks: the matrix has too many blocks");
-   const dim3 grid((unsigned)groups);
-   if (rows)       hipLaunchKernelGGL((quantize_rows_kernel<DT, CODE>), grid, dim3(256), 0, stream, p);
-   else if (whole) hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, true>), grid, dim3(256), 0, stream, p);
-   else            hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, false>), grid, dim3(256), 0, stream, p);
-   OCH_CHECK_LAUNCH();
+   if (!rows && groups > 0xFFFFFFFFull) return set_error("quantize_blocks: the matrix has too many blocks");
+   for (p.first = 0; p.first < groups; p.first += most_groups(256))
+   {  const uint64_t left = groups - p.first;
+      const dim3 grid((unsigned)(left < most_groups(256) ? left : most_groups(256)));
+      if (rows)       hipLaunchKernelGGL((quantize_rows_kernel<DT, CODE>), grid, dim3(256), 0, stream, p);
+      else if (whole) hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, true>), grid, dim3(256), 0, stream, p);
+      else            hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, false>), grid, dim3(256), 0, stream, p);
+      OCH_CHECK_LAUNCH();
+   }
    return 0;
 }
 

@@ -50,7 +50,7 @@ struct NormParams
 {
    const char *X, *R, *W; char *H, *Y; float *S, *rstd;
    int64_t  ldX, ldR, ldH, ldY, ldS;    /* in elements */
-   int64_t  n, rows;
+   int64_t  n, rows, first;             /* first: workgroup 0's place in the whole */
    float    eps, inverse;               /* inverse: 1 / n */
    int      w_float;                    /* the weights are float (else the type of X) */
 };
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_long_kernel(const NormP
 {
    typedef typename Wide<DT>::E E;
    __shared__ float part[OCH_NORM_THREADS / 64];
-   const int64_t row = blockIdx.x;
+   const int64_t row = p.first + blockIdx.x;
    const E *x = reinterpret_cast<const E *>(p.X) + row * p.ldX, *r = reinterpret_cast<const E *>(p.R) + row * p.ldR;
    E *h = reinterpret_cast<E *>(p.H) + row * p.ldH;
    float sum = 0;
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams
 {
    typedef typename Wide<DT>::E E;
    __shared__ float part[T * norm_rows(T) / 64];
-   const int64_t wanted = (int64_t)blockIdx.x * norm_rows(T) + threadIdx.x / T;
+   const int64_t wanted = (p.first + blockIdx.x) * norm_rows(T) + threadIdx.x / T;
    const bool live = wanted < p.rows;
    const int64_t row = live ? wanted : p.rows - 1;
    const int first = (int)(threadIdx.x % T) * 8, n = live ? (int)p.n : 0;      /* a group without a row: no element is valid */
@@ -201,22 +201,29 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams
    needs no barrier, but from there on more threads than vectors. 2^26 bfloat16 values with the residual stream, to codes:
       8192 features: 512 threads x 2 vectors 86.0 us, 256 x 4 90.2, 64 x 16 far behind;   16384: 512 x 4 91 us, 256 x 8 101;
       4096: 256 x 2 84.9 us, 512 x 1 83.4, but 48 against 58 without the residual stream;   5003 float: 256 x 3 15.3, 512 x 2 16.7 */
-template <int DT, int CODE> static int norm_launch(const NormParams &p, hipStream_t stream)
+template <int DT, int CODE> static int norm_launch(NormParams p, hipStream_t stream)
 {
-#define OCH_GO(T, V) hipLaunchKernelGGL((norm_kernel<DT, CODE, T, V>), dim3((unsigned)((p.rows + norm_rows(T) - 1) / norm_rows(T))), dim3(T * norm_rows(T)), 0, stream, p)
-   if (p.n <= 128)        OCH_GO(16, 1);
-   else if (p.n <= 256)   OCH_GO(16, 2);
-   else if (p.n <= 512)   OCH_GO(64, 1);
-   else if (p.n <= 1024)  OCH_GO(64, 2);
-   else if (p.n <= 2048)  OCH_GO(256, 1);
-   else if (p.n <= 4096)  OCH_GO(256, 2);
-   else if (p.n <= 6144)  OCH_GO(256, 3);
-   else if (p.n <= 8192)  OCH_GO(512, 2);
-   else if (p.n <= 16384) OCH_GO(512, 4);
-   else hipLaunchKernelGGL((norm_long_kernel<DT, CODE>), dim3((unsigned)p.rows), dim3(OCH_NORM_THREADS), 0, stream, p);
+   auto go = [&](auto kernel, int rows, int threads) -> int
+   {  const uint64_t groups = ((uint64_t)p.rows + rows - 1) / rows;
+      for (p.first = 0; (uint64_t)p.first < groups; p.first += most_groups(threads))
+      {  const uint64_t left = groups - p.first;
+         hipLaunchKernelGGL(kernel, dim3((unsigned)(left < most_groups(threads) ? left : most_groups(threads))), dim3(threads), 0, stream, p);
+         OCH_CHECK_LAUNCH();
+      }
+      return 0;
+   };
+#define OCH_GO(T, V) go(norm_kernel<DT, CODE, T, V>, norm_rows(T), T * norm_rows(T))
+   if (p.n <= 128)   return OCH_GO(16, 1);
+   if (p.n <= 256)   return OCH_GO(16, 2);
+   if (p.n <= 512)   return OCH_GO(64, 1);
+   if (p.n <= 1024)  return OCH_GO(64, 2);
+   if (p.n <= 2048)  return OCH_GO(256, 1);
+   if (p.n <= 4096)  return OCH_GO(256, 2);
+   if (p.n <= 6144)  return OCH_GO(256, 3);
+   if (p.n <= 8192)  return OCH_GO(512, 2);
+   if (p.n <= 16384) return OCH_GO(512, 4);
 #undef OCH_GO
-   OCH_CHECK_LAUNCH();
-   return 0;
+   return go(norm_long_kernel<DT, CODE>, 1, OCH_NORM_THREADS);
 }
 
 /* ---- gradients ------------------------------------------------------------------------------------------------------ */
