@@ -3,7 +3,7 @@
  * Four waves own 64 x 64 of the tile each. A slab of 128 k of both operands and the slab's scales pass through registers
  * to one of two LDS buffers: the loads of slab s + 1 are issued before the matrix instructions of slab s and stored behind
  * them, one barrier per slab, two workgroups per compute unit. Chunks of 16 bytes are single loads whatever their
- * alignment; at the matrix's border they are loaded byte by byte.
+ * alignment; at the matrix's border they are put together from two that overlap.
  *
  * ROWS: the scale of A differs between the rows of a wave (blockA = 1): a multiplication more per element and slab. */
 #pragma once
@@ -25,6 +25,13 @@ __device__ __forceinline__ void f8_tile_of(uint32_t id, uint32_t tiles_m, uint32
    tm = first + in % height; tn = in / height;
 }
 
+typedef uint64_t f8_u64_any __attribute__((aligned(1)));
+typedef uint32_t f8_u32_any __attribute__((aligned(1)));
+static __device__ __forceinline__ och_u32x4 f8_pair(uint64_t lo, uint64_t hi)
+{  och_u32x4 v;
+   v.x = (uint32_t)lo; v.y = (uint32_t)(lo >> 32); v.z = (uint32_t)hi; v.w = (uint32_t)(hi >> 32);
+   return v;
+}
 /* 16 bytes moved towards their start by `by` bytes (16 or more: zero), zeros behind */
 static __device__ __forceinline__ och_u32x4 f8_shift(och_u32x4 v, uint32_t by)
 {  uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
@@ -33,8 +40,7 @@ static __device__ __forceinline__ och_u32x4 f8_shift(och_u32x4 v, uint32_t by)
    lo = bits ? (lo >> bits | hi << (64 - bits)) : lo;
    hi >>= bits;
    if (by >= 16) lo = hi = 0;
-   v.x = (uint32_t)lo; v.y = (uint32_t)(lo >> 32); v.z = (uint32_t)hi; v.w = (uint32_t)(hi >> 32);
-   return v;
+   return f8_pair(lo, hi);
 }
 /* a chunk of which the first `valid` bytes exist (none when valid <= 0), the others zero; `length`: bytes of the run of
    memory that it ends (from 16 on, the 16 bytes up to its end are one load) */
@@ -43,14 +49,17 @@ static __device__ __forceinline__ och_u32x4 f8_border_chunk(const uint8_t *at, i
    och_u32x4 v = { 0, 0, 0, 0 };
    if (valid >= 16) v = *reinterpret_cast<const och_u32x4_any *>(at);
    else if (valid > 0 && length >= 16) v = f8_shift(*reinterpret_cast<const och_u32x4_any *>(at + valid - 16), (uint32_t)(16 - valid));
+   else if (valid >= 8)
+   {  const uint64_t lo = *reinterpret_cast<const f8_u64_any *>(at), hi = *reinterpret_cast<const f8_u64_any *>(at + valid - 8);
+      v = f8_pair(lo, valid > 8 ? hi >> (64 - 8 * (uint32_t)(valid - 8)) : 0);
+   }
+   else if (valid >= 4)
+   {  const uint64_t lo = *reinterpret_cast<const f8_u32_any *>(at), hi = *reinterpret_cast<const f8_u32_any *>(at + valid - 4);
+      v = f8_pair(lo | hi >> (32 - 8 * (uint32_t)(valid - 4)) << 32, 0);
+   }
    else if (valid > 0)
-   {  uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-      for (int e = 0; e < valid; e++)
-      {  const uint64_t b = at[e];
-         if (e < 8) lo |= b << (8 * e); else hi |= b << (8 * (e - 8));
-      }
-      v.x = (uint32_t)lo; v.y = (uint32_t)(lo >> 32); v.z = (uint32_t)hi; v.w = (uint32_t)(hi >> 32);
+   {  const uint32_t half = (uint32_t)valid / 2, last = (uint32_t)valid - 1;      /* the first, the second or last, the last */
+      v.x = at[0] | (uint32_t)at[half] << 8 * half | (uint32_t)at[last] << 8 * last;
    }
    return v;
 }

@@ -417,6 +417,7 @@ template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipSt
    else if (p.n <= 4096)  OCH_GO(256, 2);
    else if (p.n <= 6144)  OCH_GO(256, 3);
    else if (p.n <= 8192)  OCH_GO(512, 2);
+   else if (p.n <= 16384) OCH_GO(1024, 2);
    else hipLaunchKernelGGL((norm_grad_long_kernel<DT>), dim3((unsigned)groups), dim3(OCH_NORM_THREADS), 0, stream, p);
 #undef OCH_GO
    OCH_CHECK_LAUNCH();
