@@ -10,28 +10,60 @@
 
 namespace och {
 
-/* adds the shares of K in order and finishes the elements: one thread per element of C */
+/* adds the shares of K in order and finishes the elements: four rows of a column per thread, eight planes' loads under way
+   together */
 template <int DT> __global__ __launch_bounds__(256) void gemm_f8_join_kernel(const F8GemmParams p, uint32_t shares)
 {
-   const uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x, mn = (uint64_t)p.M * p.N;
-   if (e >= mn) return;
-   float s = 0;
-   for (uint32_t t = 0; t < shares; t++) s += p.partial[(size_t)t * mn + e];
-   const uint32_t n = (uint32_t)(e / p.M), m = (uint32_t)(e - (uint64_t)n * p.M);
-   f8_finish<DT>(p.C, (int64_t)m + (int64_t)n * p.ldC, s, p.alpha, p.beta);
+   const uint32_t pitch = f8_plane_pitch(p.M);
+   const uint64_t q = (uint64_t)blockIdx.x * 256 + threadIdx.x, plane = (uint64_t)pitch * p.N;
+   const uint32_t n = (uint32_t)(q / (pitch / 4)), m = (uint32_t)(q % (pitch / 4)) * 4;
+   if (n >= p.N) return;
+   och_f32x4v s = { 0, 0, 0, 0 };
+   for (uint32_t t = 0; t < shares; t += 8)
+   {  och_f32x4v v[8];
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) v[u] = *reinterpret_cast<const och_f32x4v *>(p.partial + (t + u < shares ? t + u : shares - 1) * plane + 4 * q);
+#pragma unroll
+      for (int u = 0; u < 8; u++) asm volatile("" : "+v"(v[u]));      /* all eight, before the first is waited for */
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) if (t + u < shares) s += v[u];
+   }
+   f8_finish4<DT>(p.C, (int64_t)m + (int64_t)n * p.ldC, s, p.alpha, p.beta, p.M - m);
 }
 
-/* A product on 128 x 128 tiles. Fewer tiles than half the compute units: K is cut into shares of at least four blocks, as
-   many as fill the two workgroups of every compute unit and as the workspace holds planes. */
+/* Shares of K for a product of few tiles: what takes the least time by these figures, in microseconds. A block of 128 k
+   takes a tile 1.0 (float results: 1.5; operands that cannot be pipelined: 3.4), half as much again where two workgroups share
+   a compute unit; the second kernel 2.5, and a plane 0.05 and its bytes written and read at 5 TB/s. To bfloat16, 1024 x 1024 x
+   4096: one share 37.6 us, four 21.3, eight 24.5; 2048 x 1024 x 1024: one share 13.7, two 21.0; 524 x 121 x 10112: twelve shares
+   16.0, twenty 14.4, forty 16.8. Blocks per share at the least of blocks * slab + blocks of K / blocks * plane, and the numbers
+   of shares that fill every unit once and twice, are compared with one. */
+static uint64_t gemm_f8_shares(uint64_t tiles, uint64_t slabs, uint64_t plane_bytes, uint64_t units, bool wide, bool piped)
+{
+   uint64_t best = 1, most = 2 * units / tiles;
+   const uint64_t fit = OCH_GEMM_WORKSPACE / plane_bytes;
+   if (most > slabs) most = slabs;
+   if (most > fit) most = fit;
+   const double slab = !piped ? 3.4 : wide ? 1.5 : 1.0, plane = 0.05 + (double)plane_bytes * 2 / 5e6;
+   double least = (double)slabs * slab * (tiles > units ? 1.5 : 1.0);
+   const uint64_t blocks = 1 + (uint64_t)sqrt((double)slabs * plane / slab);
+   const uint64_t tries[4] = { (slabs + blocks - 1) / blocks, blocks > 1 ? (slabs + blocks - 2) / (blocks - 1) : most, units / tiles, most };
+   for (int i = 0; i < 4; i++)
+   {  const uint64_t s = tries[i] < most ? tries[i] : most;
+      if (s < 2) continue;
+      const double time = (double)((slabs + s - 1) / s) * slab * (tiles * s > units ? 1.5 : 1.0) + 2.5 + (double)s * plane;
+      if (time < least) { least = time; best = s; }
+   }
+   return best;
+}
+
+/* A product on 128 x 128 tiles, K cut into shares where that is quicker */
 static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc, hipStream_t stream)
 {
    p.tiles_m = (p.M + OCH_F8_TILE - 1) / OCH_F8_TILE; p.tiles_n = (p.N + OCH_F8_TILE - 1) / OCH_F8_TILE;
    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n, slabs = ((uint64_t)p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB, units = (uint64_t)gemm_compute_units();
    if (tiles > most_groups(OCH_F8_TILE_THREADS)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
-   uint64_t shares = tiles * 2 <= units ? 2 * units / tiles : 1;
-   if (shares > slabs / 4) shares = slabs / 4;
-   const uint64_t fit = OCH_GEMM_WORKSPACE / ((uint64_t)p.M * p.N * sizeof(float));
-   if (shares > fit) shares = fit;
+   const bool piped = (akc || p.M >= 16) && (bkc || p.N >= 16) && p.ldA < (1 << 24) && p.ldB < (1 << 24);
+   uint64_t shares = gemm_f8_shares(tiles, slabs, (uint64_t)f8_plane_pitch(p.M) * p.N * sizeof(float), units, p.dtypeC == OCH_FLOAT, piped);
    if (shares >= 2)
    {  char *ws;
       if (stream_gemm_workspace(stream, &ws) != 0) return -1;
@@ -44,7 +76,7 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
    const int status = e5a ? (e5b ? gemm_f8_tile_55(p, akc, bkc, grid, stream) : gemm_f8_tile_54(p, akc, bkc, grid, stream))
                           : (e5b ? gemm_f8_tile_45(p, akc, bkc, grid, stream) : gemm_f8_tile_44(p, akc, bkc, grid, stream));
    if (status != 0 || p.share_slabs == 0) return status;
-   const dim3 join((unsigned)(((uint64_t)p.M * p.N + 255) / 256));
+   const dim3 join((unsigned)(((uint64_t)f8_plane_pitch(p.M) / 4 * p.N + 255) / 256));
    if (p.dtypeC == OCH_FLOAT)     hipLaunchKernelGGL(gemm_f8_join_kernel<OCH_FLOAT>, join, dim3(256), 0, stream, p, (uint32_t)shares);
    else if (p.dtypeC == OCH_HALF) hipLaunchKernelGGL(gemm_f8_join_kernel<OCH_HALF>, join, dim3(256), 0, stream, p, (uint32_t)shares);
    else                           hipLaunchKernelGGL(gemm_f8_join_kernel<OCH_BFLOAT16>, join, dim3(256), 0, stream, p, (uint32_t)shares);

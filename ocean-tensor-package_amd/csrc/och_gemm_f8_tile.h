@@ -286,7 +286,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
       if (more) stash(lds + (turn ^ 1) * BUF);
       __syncthreads();
    }
-   /* the tile leaves through LDS, where the slabs were; a share of K as raw sums into the share's plane (M x N, dense) */
+   /* the tile leaves through LDS, where the slabs were; a share of K as raw sums into the share's plane */
    constexpr uint32_t PITCH = R * 4 + 16;
    static_assert(R * PITCH <= 2 * BUF, "the tile fits where the slabs were");
    {  char *mine = lds + (wn + lane % 16) * PITCH + (wm + 4 * (lane / 16)) * 4;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
    __syncthreads();
    if (p.share_slabs)
    {  F8GemmParams q = p;
-      q.C = reinterpret_cast<char *>(p.partial + (size_t)blockIdx.y * p.M * p.N); q.ldC = p.M; q.alpha = 1.0f; q.beta = 0.0f;
+      q.ldC = f8_plane_pitch(p.M); q.C = reinterpret_cast<char *>(p.partial + (size_t)blockIdx.y * q.ldC * p.N); q.alpha = 1.0f; q.beta = 0.0f;
       f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS>(q, lds, m0, n0);
    }
    else if (WIDE)                 f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS>(p, lds, m0, n0);
