@@ -44,30 +44,6 @@ template <bool KC> struct F8PipeLoads
    __device__ __forceinline__ void issue(int e, const char *slab, uint32_t target) const { load_to_lds(slab, offset[e], target + 1024 * e); }
 };
 
-/* COLUMNS columns of R rows of finished sums from LDS to C */
-template <int DT, int R, uint32_t PITCH, uint32_t COLUMNS, int THREADS> __device__ __forceinline__ void f8_pipe_write(const F8GemmParams &p, const char *lds, uint32_t m0, uint32_t n0)
-{
-   typedef typename Wide<DT>::E E;
-#pragma unroll 1
-   for (uint32_t q = threadIdx.x; q < COLUMNS * (R / 8); q += THREADS)
-   {  const uint32_t c = q / (R / 8), m = m0 + q % (R / 8) * 8, n = n0 + c;
-      if (m >= p.M || n >= p.N) continue;
-      const och_f32x4v *from = reinterpret_cast<const och_f32x4v *>(lds + c * PITCH + q % (R / 8) * 32);
-      const och_f32x4v lo = from[0], hi = from[1];
-      E *to = reinterpret_cast<E *>(p.C) + (int64_t)m + (int64_t)n * p.ldC;
-      const int64_t valid = (int64_t)p.M - m;
-      Wide8<DT> v;
-      if (p.beta != 0.0f) v.load(to, valid);
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-      {  float x = p.alpha * (e < 4 ? lo[e % 4] : hi[e % 4]);
-         if (p.beta != 0.0f) x = __builtin_fmaf(p.beta, v.get(e), x);
-         v.put(e, x);
-      }
-      v.store(to, valid);
-   }
-}
-
 template <bool AKC, bool BKC, bool E5A, bool E5B, bool ROWS>
 __global__ __launch_bounds__(OCH_F8_PIPE_THREADS, 2) void gemm_f8_pipe_kernel(const F8GemmParams p)
 {
@@ -221,8 +197,8 @@ __global__ __launch_bounds__(OCH_F8_PIPE_THREADS, 2) void gemm_f8_pipe_kernel(co
             for (int i = 0; i < TI; i++) *reinterpret_cast<och_f32x4v *>(mine + 16 * j * PITCH + 64 * i) = acc[i][j];
       }
       __syncthreads();
-      if (p.dtypeC == OCH_HALF) f8_pipe_write<OCH_HALF, R, PITCH, HALF, THREADS>(p, lds, m0, n0 + pass * HALF);
-      else                      f8_pipe_write<OCH_BFLOAT16, R, PITCH, HALF, THREADS>(p, lds, m0, n0 + pass * HALF);
+      if (p.dtypeC == OCH_HALF) f8_store_columns<OCH_HALF, R, PITCH, HALF, THREADS>(p, lds, m0, n0 + pass * HALF);
+      else                      f8_store_columns<OCH_BFLOAT16, R, PITCH, HALF, THREADS>(p, lds, m0, n0 + pass * HALF);
    }
 }
 

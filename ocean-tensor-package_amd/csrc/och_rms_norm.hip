@@ -284,13 +284,15 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_grad_long_kernel(const 
 }
 
 /* Rows of at most 8 T V elements: T threads keep a row in registers; a workgroup takes norm_rows(T) rows at a time,
-   in steps of the grid, and its threads' sums for dw stay in registers until its last row. T = 64: the four waves' sums meet
-   in LDS then. 16384 rows of 4096 bfloat16 features with dh: 55 us (4.8 TB/s), the last step's 3 us included. */
+   in steps of the grid, loads the next ones while it works, and its threads' sums for dw stay in registers until its last row;
+   those of rows side by side meet in LDS then. 8192 rows of 4096 bfloat16 features with dh: 51.6 us (5.2 TB/s), 55.4 without
+   the next row's loads; the second kernel's 3 us are part of it. */
 template <int DT, int T, int V>
 __global__ __launch_bounds__(T * norm_rows(T)) void norm_grad_kernel(const NormGradParams p)
 {
    typedef typename Wide<DT>::E E;
    constexpr int ROWS = norm_rows(T);
+   constexpr bool AHEAD = T < 1024;                         /* with 1024 threads there are not registers enough */
    __shared__ float part[T * ROWS / 64];
    __shared__ __align__(16) float meet[ROWS > 1 ? ROWS * T * V * 8 : 4];
    const int first = (int)(threadIdx.x % T) * 8, n = (int)p.n;
@@ -301,26 +303,47 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_grad_kernel(const NormG
 #pragma unroll
       for (int e = 0; e < 8; e++) dw[v][e] = 0;
    }
-   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.rows; row0 += (int64_t)gridDim.x * ROWS)
+   Wide8<DT> a[V], b[V], c[V];
+   float rstd;
+   bool live;
+   int64_t row;
+   /* the group's row of those that begin at row0 */
+   auto load = [&](int64_t row0)
    {  const int64_t wanted = row0 + threadIdx.x / T;
-      const bool live = wanted < p.rows;
-      const int64_t row = live ? wanted : p.rows - 1;
-      const int valid = live ? n : 0;
-      Wide8<DT> a[V], b[V], c[V];
+      live = wanted < p.rows;
+      row = live ? wanted : p.rows - 1;
 #pragma unroll
       for (int v = 0; v < V; v++)
-      {  const int at = first + v * T * 8;
-         a[v].load(reinterpret_cast<const E *>(p.dY) + row * p.lddY + at, valid - at);
-         b[v].load(reinterpret_cast<const E *>(p.H) + row * p.ldH + at, valid - at);
-         if (p.dH) c[v].load(reinterpret_cast<const E *>(p.dH) + row * p.lddH + at, valid - at);
+      {  const int at = first + v * T * 8, valid = (live ? n : 0) - at;
+         a[v].load(reinterpret_cast<const E *>(p.dY) + row * p.lddY + at, valid);
+         b[v].load(reinterpret_cast<const E *>(p.H) + row * p.ldH + at, valid);
+         if (p.dH) c[v].load(reinterpret_cast<const E *>(p.dH) + row * p.lddH + at, valid);
       }
-      const float rstd = p.rstd[row];
+      rstd = p.rstd[row];
+   };
+   const int64_t step = (int64_t)gridDim.x * ROWS;
+   int64_t row0 = (int64_t)blockIdx.x * ROWS;
+   if (AHEAD && row0 < p.rows) load(row0);
+   for (; row0 < p.rows; row0 += step)
+   {  Wide8<DT> copy[3][AHEAD ? V : 1];                     /* this row; the next one's loads are under way beside it */
+      const Wide8<DT> *dy = AHEAD ? copy[0] : a, *h = AHEAD ? copy[1] : b, *dh = AHEAD ? copy[2] : c;
+      if (!AHEAD) load(row0);
+      const float r = rstd;
+      const int valid = live ? n : 0;
+      E *to = reinterpret_cast<E *>(p.dX) + row * p.lddX;
+      const bool mine = live;
+      if (AHEAD)
+      {
+#pragma unroll
+         for (int v = 0; v < V; v++) { copy[0][AHEAD ? v : 0] = a[v]; copy[1][AHEAD ? v : 0] = b[v]; copy[2][AHEAD ? v : 0] = c[v]; }
+      }
+      if (AHEAD && row0 + step < p.rows) load(row0 + step);
       float sum = 0;
 #pragma unroll
       for (int v = 0; v < V; v++)
       {  float s = 0;
 #pragma unroll
-         for (int e = 0; e < 8; e++) s = __builtin_fmaf(a[v].get(e) * w[v][e], b[v].get(e) * rstd, s);
+         for (int e = 0; e < 8; e++) s = __builtin_fmaf(dy[v].get(e) * w[v][e], h[v].get(e) * r, s);
          sum += s;
       }
       const float mean = group_sum<T>(sum, part) * p.inverse;
@@ -330,13 +353,13 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_grad_kernel(const NormG
          Wide8<DT> o;
 #pragma unroll
          for (int e = 0; e < 8; e++)
-         {  const float u = b[v].get(e) * rstd;
-            float x = rstd * (a[v].get(e) * w[v][e] - u * mean);
-            if (p.dH) x += c[v].get(e);
+         {  const float u = h[v].get(e) * r;
+            float x = r * (dy[v].get(e) * w[v][e] - u * mean);
+            if (p.dH) x += dh[v].get(e);
             o.put(e, x);
-            dw[v][e] = __builtin_fmaf(a[v].get(e), live ? u : 0.0f, dw[v][e]);
+            dw[v][e] = __builtin_fmaf(dy[v].get(e), mine ? u : 0.0f, dw[v][e]);
          }
-         o.store(reinterpret_cast<E *>(p.dX) + row * p.lddX + at, valid - at);
+         o.store(to + at, valid - at);
       }
    }
    if (p.partial == nullptr) return;
@@ -393,13 +416,13 @@ __global__ __launch_bounds__(1024) void norm_grad_finish_kernel(const float *par
    dW[at] = s;
 }
 
-/* Workgroups: each costs n floats written and read again for dw, so as few as keep the memory busy, and their row loops long.
-   2^26 values with dw: 4096 features 55.5 us with two per compute unit, 58.6 with four; 2048 features 58.0 with four, 60.4
-   with two; 8192 features (512 threads) 56.9 with one, 59.8 with two of 256 threads. */
+/* Workgroups: each costs n floats written and read again for dw, so as few as keep the memory busy. 2^25 bfloat16 values with
+   dw: 8192 features 53.5 us with one per compute unit, 57.3 with two, 64.0 with four; 2048 features 68.2, 51.4,
+   57.0; 256 features, sixteen rows at a time, 52.8 with two, 58.3 with four. */
 template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipStream_t stream)
 {
-   const int rows_at_once = p.n <= 1024 ? 4 : 1;
-   uint64_t groups = (p.n <= 2048 ? 4 : p.n <= 6144 ? 2 : 1) * (uint64_t)gemm_compute_units();
+   const int rows_at_once = norm_rows(p.n <= 256 ? 16 : p.n <= 1024 ? 64 : OCH_NORM_THREADS);
+   uint64_t groups = (p.n <= 2048 ? 2 : 1) * (uint64_t)gemm_compute_units();
    if (groups > ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once) groups = ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once;
    p.partial = nullptr;
    if (dW)
@@ -411,7 +434,9 @@ template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipSt
       p.partial = reinterpret_cast<float *>(ws);
    }
 #define OCH_GO(T, V) hipLaunchKernelGGL((norm_grad_kernel<DT, T, V>), dim3((unsigned)groups), dim3(T * norm_rows(T)), 0, stream, p)
-   if (p.n <= 512)        OCH_GO(64, 1);
+   if (p.n <= 128)        OCH_GO(16, 1);
+   else if (p.n <= 256)   OCH_GO(16, 2);
+   else if (p.n <= 512)   OCH_GO(64, 1);
    else if (p.n <= 1024)  OCH_GO(64, 2);
    else if (p.n <= 2048)  OCH_GO(256, 1);
    else if (p.n <= 4096)  OCH_GO(256, 2);
