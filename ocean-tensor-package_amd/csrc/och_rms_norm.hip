@@ -17,8 +17,8 @@ namespace och {
 /* x of the lane that the DPP control names, added */
 template <int CTRL> __device__ __forceinline__ float dpp_add(float x)
 {  const int i = __float_as_int(x); return x + __int_as_float(__builtin_amdgcn_update_dpp(0, i, CTRL, 0xF, 0xF, true)); }
-__device__ __forceinline__ float row16_sum(float x)
-{  x = dpp_add<0xB1>(x); x = dpp_add<0x4E>(x); x = dpp_add<0x141>(x); return dpp_add<0x140>(x); }
+__device__ __forceinline__ float row8_sum(float x)  { x = dpp_add<0xB1>(x); x = dpp_add<0x4E>(x); return dpp_add<0x141>(x); }
+__device__ __forceinline__ float row16_sum(float x) { return dpp_add<0x140>(row8_sum(x)); }
 __device__ __forceinline__ float lane_float(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 /* sum over the wave, in all lanes: a fixed tree */
 __device__ __forceinline__ float wave64_sum(float x)
@@ -36,9 +36,10 @@ __device__ __forceinline__ float block_sum(float x, float *part)
    return s;
 }
 
-/* sum over the T threads that share a row (T a power of two from 16 on; BLOCK threads in all) */
+/* sum over the T threads that share a row: 8, 16, 64 or the workgroup */
 template <int T> __device__ __forceinline__ float group_sum(float x, float *part)
-{  if (T == 16) return row16_sum(x);
+{  if (T == 8) return row8_sum(x);
+   if (T == 16) return row16_sum(x);
    if (T == 64) return wave64_sum(x);
    return block_sum(x, part);
 }
@@ -200,7 +201,8 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams
 /* Threads and vectors by the row's length: as few threads as hold the row in two vectors each, because a group within a wave
    needs no barrier, but from there on more threads than vectors. 2^26 bfloat16 values with the residual stream, to codes:
       8192 features: 512 threads x 2 vectors 86.0 us, 256 x 4 90.2, 64 x 16 far behind;   16384: 512 x 4 91 us, 256 x 8 101;
-      4096: 256 x 2 84.9 us, 512 x 1 83.4, but 48 against 58 without the residual stream;   5003 float: 256 x 3 15.3, 512 x 2 16.7 */
+      4096: 256 x 2 84.9 us, 512 x 1 83.4, but 48 against 58 without the residual stream;   5003 float: 256 x 3 15.3, 512 x 2 16.7;
+   2^25 values in rows of 64, without it and without codes: 8 x 1 26.3 us, 16 x 1 39.8 */
 template <int DT, int CODE> static int norm_launch(NormParams p, hipStream_t stream)
 {
    auto go = [&](auto kernel, int rows, int threads) -> int
@@ -213,6 +215,7 @@ template <int DT, int CODE> static int norm_launch(NormParams p, hipStream_t str
       return 0;
    };
 #define OCH_GO(T, V) go(norm_kernel<DT, CODE, T, V>, norm_rows(T), T * norm_rows(T))
+   if constexpr (CODE == 0) if (p.n <= 64) return OCH_GO(8, 1);          /* (codes: sixteen threads share a block's maximum) */
    if (p.n <= 128)   return OCH_GO(16, 1);
    if (p.n <= 256)   return OCH_GO(16, 2);
    if (p.n <= 512)   return OCH_GO(64, 1);
@@ -418,10 +421,11 @@ __global__ __launch_bounds__(1024) void norm_grad_finish_kernel(const float *par
 
 /* Workgroups: each costs n floats written and read again for dw, so as few as keep the memory busy. 2^25 bfloat16 values with
    dw: 8192 features 53.5 us with one per compute unit, 57.3 with two, 64.0 with four; 2048 features 68.2, 51.4,
-   57.0; 256 features, sixteen rows at a time, 52.8 with two, 58.3 with four. */
+   57.0; 256 features, sixteen threads a row, 52.8 with two, 58.3 with four; 64 features 51.6 with eight threads a row, 133 with
+   sixteen. */
 template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipStream_t stream)
 {
-   const int rows_at_once = norm_rows(p.n <= 256 ? 16 : p.n <= 1024 ? 64 : OCH_NORM_THREADS);
+   const int rows_at_once = norm_rows(p.n <= 64 ? 8 : p.n <= 256 ? 16 : p.n <= 1024 ? 64 : OCH_NORM_THREADS);
    uint64_t groups = (p.n <= 2048 ? 2 : 1) * (uint64_t)gemm_compute_units();
    if (groups > ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once) groups = ((uint64_t)p.rows + rows_at_once - 1) / rows_at_once;
    p.partial = nullptr;
@@ -434,7 +438,8 @@ template <int DT> static int norm_grad_launch(NormGradParams p, float *dW, hipSt
       p.partial = reinterpret_cast<float *>(ws);
    }
 #define OCH_GO(T, V) hipLaunchKernelGGL((norm_grad_kernel<DT, T, V>), dim3((unsigned)groups), dim3(T * norm_rows(T)), 0, stream, p)
-   if (p.n <= 128)        OCH_GO(16, 1);
+   if (p.n <= 64)         OCH_GO(8, 1);
+   else if (p.n <= 128)   OCH_GO(16, 1);
    else if (p.n <= 256)   OCH_GO(16, 2);
    else if (p.n <= 512)   OCH_GO(64, 1);
    else if (p.n <= 1024)  OCH_GO(64, 2);

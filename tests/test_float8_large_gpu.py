@@ -71,7 +71,7 @@ def repeated(pattern, count, got):
 
 def test_more_rows_than_a_launch_has_threads(hip, stream):
     rng = np.random.default_rng(1)
-    rows, period = (1 << 28) + 33, 4099                                     # sixteen threads a row: 2^32 and more
+    rows, period = (1 << 29) + 33, 4099                                     # eight threads a row: 2^32 and more
     x = F.to_wide(rng.standard_normal((period, 1)) * 3, F.HALF)
     near = T.run_norm(stream, x, None, None, F.HALF, F.FLOAT, F.HALF)
     T.check_norm({"h": None, "rstd": near["rstd"], "y": near["y"]}, x, None, None, F.HALF, F.FLOAT, F.HALF)
