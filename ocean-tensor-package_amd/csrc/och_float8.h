@@ -44,11 +44,12 @@ template <int DT> struct Wide8
    typedef typename Wide<DT>::E E;
    static constexpr int WORDS = (int)sizeof(E) * 8 / 16;
    union { och_u32x4 raw[WORDS]; E e[8]; };
-   __device__ __forceinline__ void load(const E *at, int64_t valid)
+   /* NT: past the caches (see streams()) */
+   template <bool NT = false> __device__ __forceinline__ void load(const E *at, int64_t valid)
    {  if (valid >= 8)
-      {
+      {  const och_u32x4_any *from = reinterpret_cast<const och_u32x4_any *>(at);
 #pragma unroll
-         for (int w = 0; w < WORDS; w++) raw[w] = reinterpret_cast<const och_u32x4_any *>(at)[w];
+         for (int w = 0; w < WORDS; w++) raw[w] = NT ? __builtin_nontemporal_load(from + w) : from[w];
       }
       else
       {
@@ -56,11 +57,14 @@ template <int DT> struct Wide8
          for (int i = 0; i < 8; i++) e[i] = (i < valid) ? at[i] : (E)0.0f;
       }
    }
-   __device__ __forceinline__ void store(E *at, int64_t valid) const
+   template <bool NT = false> __device__ __forceinline__ void store(E *at, int64_t valid) const
    {  if (valid >= 8)
-      {
+      {  och_u32x4_any *to = reinterpret_cast<och_u32x4_any *>(at);
 #pragma unroll
-         for (int w = 0; w < WORDS; w++) reinterpret_cast<och_u32x4_any *>(at)[w] = raw[w];
+         for (int w = 0; w < WORDS; w++)
+         {  const och_u32x4_any x = raw[w];
+            if (NT) __builtin_nontemporal_store(x, to + w); else to[w] = x;
+         }
       }
       else
       {
@@ -132,8 +136,11 @@ template <int CODE> __device__ __forceinline__ uint32_t code4(float a, float b, 
 {  return bad ? 0x7F7F7F7Fu : code4<CODE>(a * factor, b * factor, c * factor, d * factor); }
 
 /* eight codes to memory, the first `valid` of them */
-__device__ __forceinline__ void store_codes(uint8_t *at, och_u32x2 q, int64_t valid)
-{  if (valid >= 8) *reinterpret_cast<och_u32x2_any *>(at) = q;
+template <bool NT = false> __device__ __forceinline__ void store_codes(uint8_t *at, och_u32x2 q, int64_t valid)
+{  if (valid >= 8)
+   {  const och_u32x2_any x = q;
+      if (NT) __builtin_nontemporal_store(x, reinterpret_cast<och_u32x2_any *>(at)); else *reinterpret_cast<och_u32x2_any *>(at) = x;
+   }
    else
    {
 #pragma unroll
@@ -141,6 +148,9 @@ __device__ __forceinline__ void store_codes(uint8_t *at, och_u32x2 q, int64_t va
    }
 }
 
+/* host: whether a matrix of so many bytes is moved past the caches: large ones, of which little would be found there again,
+   whose columns begin on whole cache lines, because a line that two accesses share would be moved twice */
+static inline bool streams(const void *at, uint64_t column_bytes, uint64_t bytes) { return bytes >= (32u << 20) && ((uintptr_t)at | column_bytes) % 128 == 0; }
 /* host: a launch has fewer than 2^32 threads; more work than that goes out in pieces of this many workgroups of `threads` */
 static constexpr uint64_t most_groups(uint64_t threads) { return 0xFFFFFFFFull / threads; }
 /* host: types that the three operations take */

@@ -20,10 +20,10 @@ struct QuantizeParams
 };
 
 /* Blocks of 128 x 1: sixteen lanes own a block, eight elements each, and take OCH_QUANTIZE_VECTORS blocks, sixteen apart,
-   whose loads are under way together. 8192 x 8192 bfloat16 values to codes: 36.8 us with two blocks (5.5 TB/s of reads and
-   writes), 38.5 with one, 37.1 with four. */
+   whose loads are under way together. 8192 x 8192 bfloat16 values to codes: 33.3 us (6.1 TB/s of reads and writes);
+   through the caches 36.8 with two blocks, 38.5 with one, 37.1 with four. */
 #define OCH_QUANTIZE_VECTORS 2
-template <int DT, int CODE>
+template <int DT, int CODE, bool NT>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams p)
 {
    constexpr int V = OCH_QUANTIZE_VECTORS;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
       if (!live) { j[v] = 0; kb[v] = 0; }
       i[v] = (int64_t)kb[v] * OCH_F8_BLOCK + (threadIdx.x % 16) * 8;
       valid[v] = live ? p.M - i[v] : INT64_MIN;
-      x[v].load(reinterpret_cast<const E *>(p.X) + i[v] + j[v] * p.ldX, valid[v]);
+      x[v].template load<NT>(reinterpret_cast<const E *>(p.X) + i[v] + j[v] * p.ldX, valid[v]);
    }
 #pragma unroll
    for (int v = 0; v < V; v++)
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
       och_u32x2 q;
       q.x = code4<CODE>(x[v].get(0), x[v].get(1), x[v].get(2), x[v].get(3), factor, bad);
       q.y = code4<CODE>(x[v].get(4), x[v].get(5), x[v].get(6), x[v].get(7), factor, bad);
-      store_codes(p.Q + i[v] + j[v] * p.ldQ, q, valid[v]);
+      store_codes<NT>(p.Q + i[v] + j[v] * p.ldQ, q, valid[v]);
       if (valid[v] > 0 && threadIdx.x % 16 == 0) p.S[kb[v] + j[v] * p.ldS] = scale;
    }
 }
@@ -62,9 +62,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
 /* Blocks of 1 x 128 and 128 x 128 (WHOLE): a workgroup of 256 owns 128 x 128 elements; thread t holds rows
    8 (t % 16) .. + 7 of columns t / 16 + 16 c, c = 0 .. 7. The maxima over the columns are taken in registers first, then
    over the four groups of lanes of the wave, and then the four waves' meet in LDS.
-   8192 x 4096 floats in 128 x 128 blocks: 30.4 us (5.5 TB/s), 31.6 where all sixteen threads of a column meet in LDS;
+   8192 x 4096 floats in 128 x 128 blocks: 30.0 us (5.6 TB/s), 31.6 where all sixteen threads of a column meet in LDS;
    5003 x 4001 halfs, too few for a second round of workgroups, in 1 x 128 blocks: 17.5 us (3.5 TB/s) against 19.6. */
-template <int DT, int CODE, bool WHOLE>
+template <int DT, int CODE, bool WHOLE, bool NT>
 __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams p)
 {
    typedef typename Wide<DT>::E E;
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams
    uint32_t m[WORDS];
 #pragma unroll
    for (int c = 0; c < 8; c++)
-      v[c].load(reinterpret_cast<const E *>(p.X) + i + (j0 + 16 * c) * p.ldX, j0 + 16 * c < p.N ? valid : 0);
+      v[c].template load<NT>(reinterpret_cast<const E *>(p.X) + i + (j0 + 16 * c) * p.ldX, j0 + 16 * c < p.N ? valid : 0);
 #pragma unroll
    for (int w = 0; w < WORDS; w++)
    {  m[w] = 0;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams
       q.x = code4<CODE>(v[c].get(0) * factor[0], v[c].get(1) * factor[1], v[c].get(2) * factor[2], v[c].get(3) * factor[3]);
       q.y = code4<CODE>(v[c].get(4) * factor[4], v[c].get(5) * factor[5], v[c].get(6) * factor[6], v[c].get(7) * factor[7]);
       q.x = (q.x & keep[0]) | (0x7F7F7F7Fu & ~keep[0]); q.y = (q.y & keep[1]) | (0x7F7F7F7Fu & ~keep[1]);
-      store_codes(p.Q + i + (j0 + 16 * c) * p.ldQ, q, j0 + 16 * c < p.N ? valid : 0);
+      store_codes<NT>(p.Q + i + (j0 + 16 * c) * p.ldQ, q, j0 + 16 * c < p.N ? valid : 0);
    }
    if (WHOLE) { if (threadIdx.x == 0) p.S[kb + nb * p.ldS] = scale[0]; }
    else if (tj == 0)
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams
    }
 }
 
-template <int DT, int CODE>
+template <int DT, int CODE, bool NT>
 static int quantize_launch(QuantizeParams p, bool rows, bool whole, hipStream_t stream)
 {
    const uint64_t groups = rows ? (p.blocks + 16 * OCH_QUANTIZE_VECTORS - 1) / (16 * OCH_QUANTIZE_VECTORS) : (uint64_t)p.bm * ((p.N + OCH_F8_BLOCK - 1) / OCH_F8_BLOCK);
@@ -137,9 +137,9 @@ static int quantize_launch(QuantizeParams p, bool rows, bool whole, hipStream_t 
    for (p.first = 0; p.first < groups; p.first += most_groups(256))
    {  const uint64_t left = groups - p.first;
       const dim3 grid((unsigned)(left < most_groups(256) ? left : most_groups(256)));
-      if (rows)       hipLaunchKernelGGL((quantize_rows_kernel<DT, CODE>), grid, dim3(256), 0, stream, p);
-      else if (whole) hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, true>), grid, dim3(256), 0, stream, p);
-      else            hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, false>), grid, dim3(256), 0, stream, p);
+      if (rows)       hipLaunchKernelGGL((quantize_rows_kernel<DT, CODE, NT>), grid, dim3(256), 0, stream, p);
+      else if (whole) hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, true, NT>), grid, dim3(256), 0, stream, p);
+      else            hipLaunchKernelGGL((quantize_tile_kernel<DT, CODE, false, NT>), grid, dim3(256), 0, stream, p);
       OCH_CHECK_LAUNCH();
    }
    return 0;
@@ -167,8 +167,13 @@ extern "C" int och_quantize_blocks(int dtype, int code, size_t M, size_t N, cons
    QuantizeParams p;
    p.X = (const char *)X; p.Q = (uint8_t *)Q; p.S = S; p.ldX = ldX; p.ldQ = ldQ; p.ldS = ldS; p.M = (int64_t)M; p.N = (int64_t)N;
    p.bm = (uint32_t)((M + OCH_F8_BLOCK - 1) / OCH_F8_BLOCK); p.blocks = (uint64_t)p.bm * N;
-#define OCH_GO(DT) (code == OCH_FLOAT8_E4M3 ? quantize_launch<DT, OCH_FLOAT8_E4M3>(p, rows, whole, as_stream(stream)) \
-                                            : quantize_launch<DT, OCH_FLOAT8_E5M2>(p, rows, whole, as_stream(stream)))
+   /* 8192 x 8192 bfloat16 values in blocks of 128 x 1: 33.3 us past the caches, 36.7 through them; 5003 x 4001 halfs, whose
+      columns do not begin on whole lines, 22.5 against 17.2 */
+   const size_t es = wide_size(dtype);
+   const bool nt = streams(X, ldX * es, (uint64_t)M * N * es) && streams(Q, ldQ, (uint64_t)M * N);
+#define OCH_GO_CODE(DT, CODE) (nt ? quantize_launch<DT, CODE, true>(p, rows, whole, as_stream(stream)) : quantize_launch<DT, CODE, false>(p, rows, whole, as_stream(stream)))
+#define OCH_GO(DT) (code == OCH_FLOAT8_E4M3 ? OCH_GO_CODE(DT, OCH_FLOAT8_E4M3) : OCH_GO_CODE(DT, OCH_FLOAT8_E5M2))
    return OCH_BY_WIDE(dtype, OCH_GO);
 #undef OCH_GO
+#undef OCH_GO_CODE
 }

@@ -85,13 +85,13 @@ template <int DT> __device__ __forceinline__ void load_weights(const char *W, in
 
 /* eight values of the output: rounded to the input's type, or to codes with a scale that sixteen lanes share.
    Every lane of the wave calls it (CODE != 0 exchanges maxima between lanes). */
-template <int DT, int CODE> __device__ __forceinline__ void norm_store(const NormParams &p, int64_t row, int64_t at, int64_t valid, const float *y)
+template <int DT, int CODE, bool NT> __device__ __forceinline__ void norm_store(const NormParams &p, int64_t row, int64_t at, int64_t valid, const float *y)
 {
    if constexpr (CODE == 0)
    {  Wide8<DT> o;
 #pragma unroll
       for (int e = 0; e < 8; e++) o.put(e, y[e]);
-      o.store(reinterpret_cast<typename Wide<DT>::E *>(p.Y) + at + row * p.ldY, valid);
+      o.template store<NT>(reinterpret_cast<typename Wide<DT>::E *>(p.Y) + at + row * p.ldY, valid);
    }
    else
    {  float m = 0;                                        /* a NaN stays; values behind the row's end are zero, or NaN with the row */
@@ -102,7 +102,7 @@ template <int DT, int CODE> __device__ __forceinline__ void norm_store(const Nor
       och_u32x2 q;
       q.x = code4<CODE>(y[0], y[1], y[2], y[3], factor, bad);
       q.y = code4<CODE>(y[4], y[5], y[6], y[7], factor, bad);
-      store_codes(reinterpret_cast<uint8_t *>(p.Y) + at + row * p.ldY, q, valid);
+      store_codes<NT>(reinterpret_cast<uint8_t *>(p.Y) + at + row * p.ldY, q, valid);
       if (at % OCH_F8_BLOCK == 0 && valid > 0) p.S[at / OCH_F8_BLOCK + row * p.ldS] = scale;
    }
 }
@@ -141,15 +141,15 @@ __global__ __launch_bounds__(OCH_NORM_THREADS) void norm_long_kernel(const NormP
       load_weights<DT>(p.W, p.w_float, at, p.n - at, w);
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = v.get(e) * rstd * w[e];
-      norm_store<DT, CODE>(p, row, at, p.n - at, y);
+      norm_store<DT, CODE, false>(p, row, at, p.n - at, y);
    }
 }
 
 /* Rows of at most 8 T V elements: T threads keep a row in registers, eight neighbouring elements in each of V vectors per
    thread, norm_rows(T) rows per workgroup. One pass over memory, which is what bounds it, then the instructions per element: with a
    general division for scale, factor, mean and root, 8192 rows of 8192 bfloat16 features to codes took 47.4 us, now 42.8.
-   With the residual stream in and out: 84.3 us (5.6 TB/s of reads and writes); 5003 float features: 5.2 TB/s. */
-template <int DT, int CODE, int T, int V>
+   With the residual stream in and out: 82.2 us (5.7 TB/s of reads and writes); 5003 float features: 5.4 TB/s. */
+template <int DT, int CODE, int T, int V, bool NT>
 __global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams p)
 {
    typedef typename Wide<DT>::E E;
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams
    if (p.H)
    {  E *to = reinterpret_cast<E *>(p.H) + row * p.ldH;
 #pragma unroll
-      for (int v = 0; v < V; v++) h[v].store(to + first + v * T * 8, n - first - v * T * 8);
+      for (int v = 0; v < V; v++) h[v].template store<NT>(to + first + v * T * 8, n - first - v * T * 8);
    }
    float sum = 0;
 #pragma unroll
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(T * norm_rows(T)) void norm_kernel(const NormParams
       load_weights<DT>(p.W, p.w_float, at, n - at, w);
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = h[v].get(e) * rstd * w[e];
-      norm_store<DT, CODE>(p, row, at, n - at, y);
+      norm_store<DT, CODE, NT>(p, row, at, n - at, y);
    }
 }
 
@@ -214,17 +214,22 @@ template <int DT, int CODE> static int norm_launch(NormParams p, hipStream_t str
       }
       return 0;
    };
-#define OCH_GO(T, V) go(norm_kernel<DT, CODE, T, V>, norm_rows(T), T * norm_rows(T))
+   /* the rows with a workgroup of their own can be stored past the caches: 8192 rows of 8192 features 82.2 us against 84.8 */
+   const uint64_t es = sizeof(typename Wide<DT>::E), values = (uint64_t)p.n * p.rows, ey = CODE == 0 ? es : 1;
+   const bool nt = streams(p.Y, p.ldY * ey, values * ey) && (p.H == nullptr || streams(p.H, p.ldH * es, values * es));
+#define OCH_GO(T, V) go(norm_kernel<DT, CODE, T, V, false>, norm_rows(T), T * norm_rows(T))
+#define OCH_GO_NT(T, V) (nt ? go(norm_kernel<DT, CODE, T, V, true>, 1, T) : OCH_GO(T, V))
    if constexpr (CODE == 0) if (p.n <= 64) return OCH_GO(8, 1);          /* (codes: sixteen threads share a block's maximum) */
    if (p.n <= 128)   return OCH_GO(16, 1);
    if (p.n <= 256)   return OCH_GO(16, 2);
    if (p.n <= 512)   return OCH_GO(64, 1);
    if (p.n <= 1024)  return OCH_GO(64, 2);
-   if (p.n <= 2048)  return OCH_GO(256, 1);
-   if (p.n <= 4096)  return OCH_GO(256, 2);
-   if (p.n <= 6144)  return OCH_GO(256, 3);
-   if (p.n <= 8192)  return OCH_GO(512, 2);
-   if (p.n <= 16384) return OCH_GO(512, 4);
+   if (p.n <= 2048)  return OCH_GO_NT(256, 1);
+   if (p.n <= 4096)  return OCH_GO_NT(256, 2);
+   if (p.n <= 6144)  return OCH_GO_NT(256, 3);
+   if (p.n <= 8192)  return OCH_GO_NT(512, 2);
+   if (p.n <= 16384) return OCH_GO_NT(512, 4);
+#undef OCH_GO_NT
 #undef OCH_GO
    return go(norm_long_kernel<DT, CODE>, 1, OCH_NORM_THREADS);
 }

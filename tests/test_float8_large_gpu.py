@@ -93,3 +93,46 @@ def test_more_blocks_than_a_launch_has_threads(hip, stream):
     assert repeated(q[:, 0], cols, Q.download(np.uint8)) and repeated(s[:, 0], cols, S.download(np.float32))
     for b in (X, Q, S):
         b.free()
+
+
+@pytest.mark.parametrize("bm,bn", [(128, 1), (1, 128), (128, 128)])
+@pytest.mark.parametrize("dtype", T.WIDE, ids=T.name_of)
+def test_large_aligned_matrices_are_quantized_alike(hip, stream, dtype, bm, bn):
+    """Large matrices whose columns are whole cache lines go past the caches: the same codes and scales, block for block."""
+    rng = np.random.default_rng(dtype + bn)
+    M, period, N = 4096, 256, 8320
+    x = T.wide_data(rng, period, M, dtype)
+    x[5, 100] = F.to_wide(np.array(np.nan), dtype)
+    q, s = T.run_quantize(stream, x, dtype, F.E4M3, bm, bn)
+    want = F.quantize(F.from_wide(x, dtype), bm, bn, F.E4M3)
+    T.same_codes((q, np.where(np.isnan(s), np.float32(np.nan), s)), want)
+    X, Q, S = oh.to_device(np.resize(x, (N, M)), stream), oh.DeviceBuffer(N * M, stream), oh.DeviceBuffer(4 * -(-N // bn) * -(-M // bm), stream)
+    assert X.address % 128 == 0 and Q.address % 128 == 0
+    oh.check(L.och_quantize_blocks(dtype, F.E4M3, M, N, X.ptr, M, bm, bn, Q.ptr, M, S.ptr, -(-M // bm), stream.handle))
+    assert np.array_equal(Q.download(np.uint8).reshape(N, M), np.resize(q, (N, M)))
+    got = S.download(np.float32).reshape(-(-N // bn), -(-M // bm))
+    assert np.array_equal(got, np.resize(s, got.shape), equal_nan=True)
+    for b in (X, Q, S):
+        b.free()
+
+
+@pytest.mark.parametrize("n", [2048, 3968, 5888, 8192, 16384])
+@pytest.mark.parametrize("dtype,dtype_y", [(F.BF16, F.E4M3), (F.HALF, F.HALF), (F.FLOAT, F.E5M2)])
+def test_large_aligned_norms_are_alike(hip, stream, dtype, dtype_y, n):
+    rng = np.random.default_rng(n + dtype)
+    period, rows = 33, (36 << 20) // n
+    x, r = T.wide_data(rng, period, n, dtype), T.wide_data(rng, period, n, dtype)
+    w = F.to_wide(1 + 0.2 * rng.standard_normal(n), F.FLOAT)
+    near = T.run_norm(stream, x, r, w, dtype, F.FLOAT, dtype_y)
+    T.check_norm(near, x, r, w, dtype, F.FLOAT, dtype_y)
+    coded, es, st = dtype_y != dtype, F.STORAGE[dtype]().itemsize, F.STORAGE[dtype]
+    X, R, W = oh.to_device(np.resize(x, (rows, n)), stream), oh.to_device(np.resize(r, (rows, n)), stream), oh.to_device(w, stream)
+    Y, S = oh.DeviceBuffer(rows * n * (1 if coded else es), stream), oh.DeviceBuffer(4 * rows * (n // 128), stream)
+    assert Y.address % 128 == 0 and R.address % 128 == 0
+    oh.check(L.och_rms_norm(dtype, n, rows, X.ptr, n, R.ptr, n, R.ptr, n, F.FLOAT, W.ptr, 1e-5, dtype_y, Y.ptr, n, S.ptr if coded else None, n // 128, None, stream.handle))
+    assert np.array_equal(Y.download(np.uint8 if coded else st).reshape(rows, n), np.resize(near["y"], (rows, n)))
+    assert np.array_equal(R.download(st).reshape(rows, n), np.resize(near["h"], (rows, n)))
+    if coded:
+        assert np.array_equal(S.download(np.float32).reshape(rows, n // 128), np.resize(near["s"], (rows, n // 128)))
+    for b in (X, R, W, Y, S):
+        b.free()
