@@ -21,11 +21,21 @@
 
 namespace och {
 
+#define OCH_F8_STREAM (192u << 20)      /* bytes of A from which on it is loaded past the caches, whose last level holds 256 MB */
+
 static constexpr uint32_t f8_few_waves(int TN) { return TN == 1 ? 16 : 8; }      /* at most, per workgroup: more than 16 columns need over 128 registers */
 static constexpr uint32_t f8_few_slot(int TM, int TN) { return (uint32_t)(TM + TN) * 16 * OCH_F8_SLAB + 512; }      /* codes, 64 scales of A, 64 of B */
 
+/* sixteen bytes per lane from memory to LDS as load_to_lds moves them, past the caches */
+static __device__ __forceinline__ void stream_to_lds(const char *base, uint32_t offset, uint32_t target)
+{
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(target), "v"(offset), "s"(base) : "memory");
+}
+
+/* `stream`: A is larger than what the caches could hold until the next call (28672 x 1 x 8192: 37.5 us past them, 43.1 through
+   them; A's of 60 MB that take turns in them: 12.2 and 10.7) */
 template <bool E5A, bool E5B, bool WIDE, int TM, int TN>
-__global__ __launch_bounds__(64 * f8_few_waves(TN)) void gemm_f8_few_kernel(const F8GemmParams p)
+__global__ __launch_bounds__(64 * f8_few_waves(TN)) void gemm_f8_few_kernel(const F8GemmParams p, bool stream)
 {
    typedef F8Slab<true, 32> L;
    constexpr uint32_t SLOT = f8_few_slot(TM, TN), SLOT_B = TM * 16 * OCH_F8_SLAB, SLOT_SCALES = SLOT - 512;
@@ -62,9 +72,16 @@ __global__ __launch_bounds__(64 * f8_few_waves(TN)) void gemm_f8_few_kernel(cons
 #pragma unroll
       for (int j = 0; j < TN; j++) acc[i][j] = zero;
    auto fetch = [&](uint32_t s)
-   {
+   {  if (stream)
+      {
 #pragma unroll
-      for (int e = 0; e < 2 * TM; e++) load_to_lds(rowsA + (uint64_t)s * OCH_F8_SLAB, oa[e], target + 1024 * e);
+         for (int e = 0; e < 2 * TM; e++) stream_to_lds(rowsA + (uint64_t)s * OCH_F8_SLAB, oa[e], target + 1024 * e);
+      }
+      else
+      {
+#pragma unroll
+         for (int e = 0; e < 2 * TM; e++) load_to_lds(rowsA + (uint64_t)s * OCH_F8_SLAB, oa[e], target + 1024 * e);
+      }
 #pragma unroll
       for (int e = 0; e < 2 * TN; e++) load_to_lds(rowsB + (uint64_t)s * OCH_F8_SLAB, ob[e], target + SLOT_B + 1024 * e);
       load_float_to_lds(scalesA + (int64_t)s * p.sa_k * 4, osa, target + SLOT_SCALES);
@@ -152,7 +169,7 @@ template <bool E5A, bool E5B, bool WIDE, int TM, int TN> static int gemm_f8_few_
    if (groups > most_groups(64 * waves)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
    const size_t lds = (size_t)waves * f8_few_slot(TM, TN);
    if (lds > 65536) OCH_CHECK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-   hipLaunchKernelGGL(kernel, dim3(groups), dim3(64 * waves), lds, stream, p);
+   hipLaunchKernelGGL(kernel, dim3(groups), dim3(64 * waves), lds, stream, p, (uint64_t)p.M * p.K >= OCH_F8_STREAM);
    OCH_CHECK_LAUNCH();
    return 0;
 }

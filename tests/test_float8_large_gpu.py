@@ -136,3 +136,24 @@ def test_large_aligned_norms_are_alike(hip, stream, dtype, dtype_y, n):
         assert np.array_equal(S.download(np.float32).reshape(rows, n // 128), np.resize(near["s"], (rows, n // 128)))
     for b in (X, R, W, Y, S):
         b.free()
+
+
+@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("dtype", [F.HALF, F.FLOAT], ids=T.name_of)
+def test_weights_larger_than_the_caches(hip, stream, dtype, N):
+    """Rows of A that repeat give rows of C that repeat; sums are exact in every order (few enough magnitudes to stay finite in
+    half: products below 2^6 in 17 blocks of 128, scaled by 2^-8)."""
+    rng = np.random.default_rng(N)
+    M, K, period = 98_321, 2064, 96
+    a, sa, b, sb = T.exact_case(rng, period, N, K, 1, 1)
+    sa = (sa * 2.0 ** -8).astype(np.float32)
+    want = T.run_gemm(stream, F.E4M3, F.E4M3, dtype, "T", "N", a, sa, 1, b, sb, 1)
+    T.check_gemm(want, F.E4M3, F.E4M3, dtype, a, sa, 1, b, sb, 1)
+    A, SA = oh.to_device(np.resize(a, (M, K)), stream), oh.to_device(np.resize(sa, (M, sa.shape[1])), stream)
+    B, SB, Cm = oh.to_device(b, stream), oh.to_device(sb, stream), T.Matrix(stream, M, N, F.STORAGE[dtype])
+    oh.check(L.och_gemm_scaled(F.E4M3, F.E4M3, dtype, b"T", b"N", M, N, K, 1.0, A.ptr, K, SA.ptr, sa.shape[1], 1, B.ptr, K, SB.ptr, sb.shape[1], 1, 0.0, Cm.ptr, Cm.ld,
+                               stream.handle))
+    got = Cm.read()
+    assert np.array_equal(got, np.resize(want.T, (M, N)).T)
+    for x in (A, SA, B, SB, Cm):
+        x.free()
