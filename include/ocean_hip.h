@@ -462,8 +462,8 @@ int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *dY, ptrdiff_
 /* A float result has sums as good as float additions make them. For half and bfloat16 results the 8-bit matrix            */
 /* instruction adds eight products at a time and cuts off what lies below 2^-13 of the largest of them: about 1e-4 of the  */
 /* result's norm on Gaussian operands, less than the rounding to half.                                                     */
-/* beta = 0 does not read C; K = 0 leaves beta * C. Sums are added in an order that depends on sizes, leading dimensions   */
-/* and alignment alone: results are reproducible.                                                                          */
+/* beta = 0 does not read C; K = 0 leaves beta * C. Sums are added in an order that depends on sizes, types, leading        */
+/* dimensions, alignment and the device alone: results are reproducible.                                                   */
 int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, char transB, size_t M, size_t N, size_t K, float alpha,
                     const void *A, ptrdiff_t ldA, const float *SA, ptrdiff_t ldSA, size_t blockA,
                     const void *B, ptrdiff_t ldB, const float *SB, ptrdiff_t ldSB, size_t blockB,

@@ -85,8 +85,8 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
 }
 
 /* Whether a product of aligned operands is quicker on 256 x 256 tiles (one workgroup per compute unit) than on 128 x 128
-   (two): rounds of the compute units times the work of a round over its rate. Measured rates on full rounds: 2.3 and 1.5
-   PFLOP/s. */
+   (two): rounds of the compute units times the work of a round over its rate. Measured rates on full rounds of aligned
+   operands: 2.3 and 1.5 PFLOP/s. */
 static bool gemm_f8_large(size_t M, size_t N)
 {
    const double units = gemm_compute_units(), small = (double)((M + 127) / 128) * (double)((N + 127) / 128), large = (double)((M + 255) / 256) * (double)((N + 255) / 256);

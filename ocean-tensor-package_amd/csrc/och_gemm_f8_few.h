@@ -5,16 +5,15 @@
  * A workgroup owns 16 TM rows of A and all columns; its W waves share out the slabs of 128 k (wave w takes slabs w, w + W,
  * ...), so that a few thousand waves are in flight whatever M is. The workgroups of a die (every eighth) begin at different
  * slabs, or else they would all read the same k of rows that lie a power of two apart, which one channel of the die's cache
- * serves: 8192 x 16 x 8192 14.8 us instead of 19.2. Every wave
- * has a slot of its own in LDS that loads from memory fill directly, eight rows of 128 consecutive bytes per load: with
- * fragments loaded straight into registers a load covers sixteen rows of 64 bytes, which the first-level cache serves at
- * 15 instead of 38 bytes a cycle. No wave waits for another before the end, where the waves' sums meet in LDS and are added
- * in the order of the waves. Two tiles of rows share the columns' codes where there are more than 16 columns and rows enough:
- * these come from the second-level cache once per workgroup and slab.
+ * serves: 8192 x 16 x 8192 14.8 us instead of 19.2. Every wave has a slot of its own in LDS that loads from memory fill
+ * directly, eight rows of 128 consecutive bytes per load: with fragments loaded straight into registers a load covers sixteen
+ * rows of 64 bytes, which the first-level cache serves at 15 instead of 38 bytes a cycle. No wave waits for another before the
+ * end, where the waves' sums meet in LDS and are added in the order of the waves. Two tiles of rows share the columns' codes
+ * where there are more than 16 columns and rows enough: these come from the second-level cache once per workgroup and slab.
  *
- * Measured, operands of 200 MB in turn: 14336 x 1 x 4096 10.9 us (5.4 TB/s), 8192 x 16 x 8192 11.7 us (5.8 TB/s), 8192 x 48
- * x 8192 14.9 us (4.6 TB/s); every 16 columns more cost 3 us, their codes being read by all 256 workgroups (11 TB/s from the second-level
- * cache). Two slots per wave, the next but one slab under way, change nothing at these sizes. On 128 x 128 tiles 16, 22, 22. */
+ * Measured, three sets of operands in turn: 14336 x 1 x 4096 10.9 us (5.4 TB/s), 8192 x 16 x 8192 11.9 us (5.7 TB/s), 8192 x
+ * 48 x 8192 14.8 us (4.6 TB/s). Every 16 columns more cost 1.5 to 3 us, their codes being read by all 256 workgroups. Two slots
+ * per wave, the next but one slab under way, change nothing at these sizes. On 128 x 128 tiles 16, 22 and 22 us. */
 #pragma once
 #include "och_gemm_f8_tile.h"
 #pragma clang diagnostic ignored "-Winline-asm"

@@ -7,11 +7,12 @@
  *
  * ROWS: the scale of A differs between the rows of a wave (blockA = 1): a multiplication more per element and slab.
  *
- * Float results, 4096 x 5000 x 4001 with both operands contiguous along their rows: 205 us, 0.80 PFLOP/s; to bfloat16 1.1
- * PFLOP/s. A slab takes a wave about 4200 cycles, 1024 of them in matrix instructions: 600 go into issuing its loads, 400 into
- * B's fragments, 4 x 560 into the rows, whose conversions and scaling are 1024 cycles of vector instructions, 900 into waiting
- * for the loads and storing them. Loads and stores spread over the rows, or 256 x 128 tiles filled straight from memory, gain
- * nothing or 8 % on full rounds: with two workgroups per unit the clock falls from 1.9 to 1.5 GHz, power bounds it. */
+ * Float results, 4096 x 5000 x 4001 with both operands contiguous along their rows: 205 us, 0.80 PFLOP/s; unaligned 11136 x
+ * 2832 x 8716 to bfloat16: 498 us, 1.1 PFLOP/s. With float results a slab takes a wave about 4200 cycles, 1024 of them in
+ * matrix instructions: 600 go into issuing its loads, 400 into B's fragments, 4 x 560 into the rows, whose conversions and
+ * scaling are 1024 cycles of vector instructions, 900 into waiting for the loads and storing them. Loads and stores spread
+ * over the rows, or 256 x 128 tiles filled straight from memory, gain nothing or 8 % on full rounds: with two workgroups per
+ * unit the clock falls from 1.9 to 1.5 GHz, power bounds it. */
 #pragma once
 #include "och_gemm_f8.h"
 
