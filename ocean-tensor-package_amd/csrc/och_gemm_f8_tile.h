@@ -7,12 +7,16 @@
  *
  * ROWS: the scale of A differs between the rows of a wave (blockA = 1): a multiplication more per element and slab.
  *
+ * A wave that multiplies goes before one that loads, stores or waits on the same SIMD, and the loads are issued in the first
+ * row's step, behind the reads of the first fragments. 4096^3 to float: 156 -> 149 us with both operands contiguous along their
+ * rows, 148 -> 133 contiguous along k with one scale of A per 128 rows; 4096 x 4096 x 4100, unaligned, to bfloat16 117 -> 112.
+ *
  * Float results, 4096 x 5000 x 4001 with both operands contiguous along their rows: 205 us, 0.80 PFLOP/s; unaligned 11136 x
  * 2832 x 8716 to bfloat16: 498 us, 1.1 PFLOP/s. With float results a slab takes a wave about 4200 cycles, 1024 of them in
  * matrix instructions: 600 go into issuing its loads, 400 into B's fragments, 4 x 560 into the rows, whose conversions and
  * scaling are 1024 cycles of vector instructions, 900 into waiting for the loads and storing them. Loads and stores spread
- * over the rows, or 256 x 128 tiles filled straight from memory, gain nothing or 8 % on full rounds: with two workgroups per
- * unit the clock falls from 1.9 to 1.5 GHz, power bounds it. */
+ * over the rows gain nothing, 256 x 128 tiles filled straight from memory 8 % on full rounds: with two workgroups per unit the
+ * clock falls from 1.9 to 1.5 GHz, power bounds it. */
 #pragma once
 #include "och_gemm_f8.h"
 
@@ -241,7 +245,6 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
          __syncthreads();
       }
       const bool more = s + 1 < piped;
-      if (more) { la.load(p.ldA); lb.load(p.ldB); ls = next_scale(); }
       F8Operand<WIDE> b[4]; float t[4];
       {  och_i32x8 c[4];
 #pragma unroll
@@ -255,6 +258,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
             __builtin_amdgcn_sched_barrier(0);
          }
       }
+      __builtin_amdgcn_s_setprio(1);
       /* step i: row i is multiplied while the sums of row i - 1 are scaled and added and the fragment of row i + 1 is read
          and made an operand. The fences keep the compiler from collecting more rows than registers hold. */
       F8Operand<WIDE> a;
@@ -266,6 +270,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
       {  och_i32x8 codes; F8Operand<WIDE> next = a; och_f32x4v rs;
          if (ROWS && i > 0) rs = *reinterpret_cast<const och_f32x4v *>(sA + wm + 16 * (i > 0 ? i - 1 : 0) + 4 * (lane / 16));
          if (i < 3) codes = f8_fragment<AKC, R>(buf, wm + 16 * (i + 1));
+         if (i == 0 && more) { la.load(p.ldA); lb.load(p.ldB); ls = next_scale(); }
          if (i < 4)
             f8_row<E5A, E5B, 4>(a, b, part[i % 2]);
          if (i > 0)
@@ -290,6 +295,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
          a = next;
          __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (more) stash(lds + (turn ^ 1) * BUF);
       __syncthreads();
    }
