@@ -12,7 +12,7 @@
  * rows, 148 -> 133 contiguous along k with one scale of A per 128 rows; 4096 x 4096 x 4100, unaligned, to bfloat16 117 -> 112.
  *
  * Float results, 4096 x 5000 x 4001 with both operands contiguous along their rows: 205 us, 0.80 PFLOP/s; unaligned 11136 x
- * 2832 x 8716 to bfloat16: 498 us, 1.1 PFLOP/s. With float results a slab takes a wave about 4200 cycles, 1024 of them in
+ * 2832 x 8716 to bfloat16: 477 us, 1.2 PFLOP/s. With float results a slab takes a wave about 4200 cycles, 1024 of them in
  * matrix instructions: 600 go into issuing its loads, 400 into B's fragments, 4 x 560 into the rows, whose conversions and
  * scaling are 1024 cycles of vector instructions, 900 into waiting for the loads and storing them. Loads and stores spread
  * over the rows gain nothing, 256 x 128 tiles filled straight from memory 8 % on full rounds: with two workgroups per unit the
