@@ -492,6 +492,8 @@ extern "C" int och_rms_norm(int dtype, size_t n, size_t rows, const void *X, ptr
    const size_t es = wide_size(dtype);
    if ((uintptr_t)X % es || (uintptr_t)R % es || (uintptr_t)H % es || (!code && (uintptr_t)Y % es) || (uintptr_t)S % 4 || (uintptr_t)rstd % 4)
       return set_error("rms_norm: misaligned pointer");
+   if (H != nullptr && ((H == X && ldH != ldX) || (H == R && ldH != ldR))) return set_error("rms_norm: a sum in place needs its operand's leading dimension");
+   if (Y == X && (code || R != nullptr || ldY != ldX)) return set_error("rms_norm: the output can take X's place only without a residual, in X's type and with its leading dimension");
    NormParams p;
    p.X = (const char *)X; p.R = (const char *)R; p.W = (const char *)W; p.H = (char *)H; p.Y = (char *)Y; p.S = S; p.rstd = rstd;
    p.ldX = ldX; p.ldR = ldR; p.ldH = ldH; p.ldY = ldY; p.ldS = ldS; p.n = (int64_t)n; p.rows = (int64_t)rows; p.eps = eps; p.inverse = 1.0f / (float)n; p.w_float = (dtype_w == OCH_FLOAT);
@@ -515,6 +517,7 @@ extern "C" int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *d
       return set_error("rms_norm_grad: a leading dimension is smaller than the row (n = %zu)", n);
    const size_t es = wide_size(dtype);
    if ((uintptr_t)dY % es || (uintptr_t)H % es || (uintptr_t)dH % es || (uintptr_t)dX % es || (uintptr_t)rstd % 4) return set_error("rms_norm_grad: misaligned pointer");
+   if ((dX == dY && lddX != lddY) || (dX == dH && lddX != lddH)) return set_error("rms_norm_grad: dX in the place of dY or dH needs its leading dimension");
    NormGradParams p;
    p.dY = (const char *)dY; p.H = (const char *)H; p.W = (const char *)W; p.dH = (const char *)dH; p.dX = (char *)dX; p.rstd = rstd; p.partial = nullptr;
    p.lddY = lddY; p.ldH = ldH; p.lddH = lddH; p.lddX = lddX; p.n = (int64_t)n; p.rows = (int64_t)rows; p.inverse = 1.0f / (float)n; p.w_float = (dtype_w == OCH_FLOAT);

@@ -124,3 +124,14 @@ def test_oracle_rounds_to_the_nearest_code(code):
     assert np.array_equal(F.encode(middle, code) % 2, np.zeros(len(middle)))        # ties to the even code
     assert np.array_equal(F.encode(np.nextafter(middle, 1e9), code), np.arange(1, len(positive)))
     assert np.array_equal(F.encode(np.nextafter(middle, 0), code), np.arange(0, len(positive) - 1))
+
+
+def test_refusals_of_operations_in_place():
+    other = C.c_void_p(0x10000)
+    refused(norm(R=other, ldR=256, H=P, ldH=264, Y=C.c_void_p(0x20000)), "in place")
+    refused(norm(R=other, ldR=256, H=other, ldH=264, Y=C.c_void_p(0x20000)), "in place")
+    refused(norm(), "X's place")                                       # codes over X
+    refused(norm(dtype_y=F.BF16, ldY=264), "X's place")
+    refused(norm(dtype_y=F.BF16, R=other, ldR=256, H=other, ldH=256), "X's place")
+    refused(grad(lddX=264), "place of dY")
+    refused(grad(dY=other, dH=P, lddH=256, lddX=264), "place of dY")
