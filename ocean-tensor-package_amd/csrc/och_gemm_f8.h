@@ -29,10 +29,10 @@ struct F8GemmParams
 };
 /* rows of a plane of partial sums: whole groups of four */
 __host__ __device__ static inline uint32_t f8_plane_pitch(uint32_t M) { return (M + 3) & ~3u; }
-int gemm_f8_tile_44(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
-int gemm_f8_tile_45(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
-int gemm_f8_tile_54(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
-int gemm_f8_tile_55(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_44(const F8GemmParams &p, bool akc, bool bkc, bool pair, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_45(const F8GemmParams &p, bool akc, bool bkc, bool pair, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_54(const F8GemmParams &p, bool akc, bool bkc, bool pair, dim3 grid, hipStream_t stream);
+int gemm_f8_tile_55(const F8GemmParams &p, bool akc, bool bkc, bool pair, dim3 grid, hipStream_t stream);
 int gemm_f8_pipe_44(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);
 int gemm_f8_pipe_45(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);
 int gemm_f8_pipe_54(const F8GemmParams &p, bool akc, bool bkc, hipStream_t stream);

@@ -33,25 +33,29 @@ template <int DT> __global__ __launch_bounds__(256) void gemm_f8_join_kernel(con
 
 /* Shares of K for a product of few tiles: what takes the least time by these figures, in microseconds. A block of 128 k
    takes a tile 1.0 (float results: 1.5; operands that cannot be pipelined: 3.4), half as much again where two workgroups share
-   a compute unit; the second kernel 2.5, and a plane 0.05 and its bytes written and read at 5 TB/s. To bfloat16, 1024 x 1024 x
+   a compute unit; the second kernel 4, and a plane 0.05 and its bytes written and read at 5 TB/s. To bfloat16, 1024 x 1024 x
    4096: one share 37.6 us, four 21.3, eight 24.5; 2048 x 1024 x 1024: one share 13.7, two 21.0; 524 x 121 x 10112: twelve shares
-   16.0, twenty 14.4, forty 16.8. Blocks per share at the least of blocks * slab + blocks of K / blocks * plane, and the numbers
-   of shares that fill every unit once and twice, are compared with one. */
-static uint64_t gemm_f8_shares(uint64_t tiles, uint64_t slabs, uint64_t plane_bytes, uint64_t units, bool wide, bool piped)
+   16.0, twenty 14.4, forty 16.8. Pairs of groups on a tile work like two workgroups on a unit and need no plane of their own.
+   Blocks per share at the least of blocks * slab + blocks of K / blocks * plane, and the numbers of shares that fill every unit
+   once and twice, are compared with one. */
+static uint64_t gemm_f8_shares(uint64_t tiles, uint64_t slabs, uint64_t plane_bytes, uint64_t units, bool wide, bool piped, bool can_pair, bool *pair)
 {
    uint64_t best = 1, most = 2 * units / tiles;
    const uint64_t fit = OCH_GEMM_WORKSPACE / plane_bytes;
    if (most > slabs) most = slabs;
    if (most > fit) most = fit;
    const double slab = !piped ? 3.4 : wide ? 1.5 : 1.0, plane = 0.05 + (double)plane_bytes * 2 / 5e6;
-   double least = (double)slabs * slab * (tiles > units ? 1.5 : 1.0);
    const uint64_t blocks = 1 + (uint64_t)sqrt((double)slabs * plane / slab);
-   const uint64_t tries[4] = { (slabs + blocks - 1) / blocks, blocks > 1 ? (slabs + blocks - 2) / (blocks - 1) : most, units / tiles, most };
-   for (int i = 0; i < 4; i++)
-   {  const uint64_t s = tries[i] < most ? tries[i] : most;
-      if (s < 2) continue;
-      const double time = (double)((slabs + s - 1) / s) * slab * (tiles * s > units ? 1.5 : 1.0) + 2.5 + (double)s * plane;
-      if (time < least) { least = time; best = s; }
+   const uint64_t tries[6] = { 1, (slabs + blocks - 1) / blocks, blocks > 1 ? (slabs + blocks - 2) / (blocks - 1) : most, (slabs + 2 * blocks - 1) / (2 * blocks), units / tiles, most };
+   double least = INFINITY;
+   *pair = false;
+   for (int i = 0; i < 6; i++)
+   {  const uint64_t s = tries[i] < most ? tries[i] : most, own = s < 2 ? slabs : (slabs + s - 1) / s;
+      if (s < 2 && i > 0) continue;
+      const double join = s < 2 ? 0 : 4.0 + (double)s * plane;
+      const double single = (double)own * slab * (tiles * s > units ? 1.5 : 1.0) + join, twin = (double)((own + 1) / 2) * slab * 1.5 + 0.5 + join;
+      if (single < least) { least = single; best = s < 2 ? 1 : s; *pair = false; }
+      if (can_pair && own > 1 && tiles * s <= units && twin < least) { least = twin; best = s < 2 ? 1 : s; *pair = true; }
    }
    return best;
 }
@@ -63,7 +67,8 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n, slabs = ((uint64_t)p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB, units = (uint64_t)gemm_compute_units();
    if (tiles > most_groups(OCH_F8_TILE_THREADS)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
    const bool piped = (akc || p.M >= 16) && (bkc || p.N >= 16) && p.ldA < (1 << 24) && p.ldB < (1 << 24);
-   uint64_t shares = gemm_f8_shares(tiles, slabs, (uint64_t)f8_plane_pitch(p.M) * p.N * sizeof(float), units, p.dtypeC == OCH_FLOAT, piped);
+   bool pair;
+   uint64_t shares = gemm_f8_shares(tiles, slabs, (uint64_t)f8_plane_pitch(p.M) * p.N * sizeof(float), units, p.dtypeC == OCH_FLOAT, piped, piped && p.K % OCH_F8_SLAB == 0, &pair);
    if (shares >= 2)
    {  char *ws;
       if (stream_gemm_workspace(stream, &ws) != 0) return -1;
@@ -73,8 +78,8 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
    }
    else shares = 1;
    const dim3 grid((unsigned)tiles, (unsigned)shares);
-   const int status = e5a ? (e5b ? gemm_f8_tile_55(p, akc, bkc, grid, stream) : gemm_f8_tile_54(p, akc, bkc, grid, stream))
-                          : (e5b ? gemm_f8_tile_45(p, akc, bkc, grid, stream) : gemm_f8_tile_44(p, akc, bkc, grid, stream));
+   const int status = e5a ? (e5b ? gemm_f8_tile_55(p, akc, bkc, pair, grid, stream) : gemm_f8_tile_54(p, akc, bkc, pair, grid, stream))
+                          : (e5b ? gemm_f8_tile_45(p, akc, bkc, pair, grid, stream) : gemm_f8_tile_44(p, akc, bkc, pair, grid, stream));
    if (status != 0 || p.share_slabs == 0) return status;
    const dim3 join((unsigned)(((uint64_t)f8_plane_pitch(p.M) / 4 * p.N + 255) / 256));
    if (p.dtypeC == OCH_FLOAT)     hipLaunchKernelGGL(gemm_f8_join_kernel<OCH_FLOAT>, join, dim3(256), 0, stream, p, (uint32_t)shares);

@@ -5,6 +5,10 @@
  * them, one barrier per slab, two workgroups per compute unit. Chunks of 16 bytes are single loads whatever their
  * alignment; at the matrix's border they are put together from two that overlap.
  *
+ * PAIR: where there are no more tiles than compute units, two groups of four waves share a tile, each with its half of K and
+ * LDS of its own, as two workgroups would; their sums meet in LDS. Only for K of whole slabs, all pipelined: the groups have
+ * one barrier in common. 2048 x 2048 x 4096 to bfloat16 40 -> 28.5 us, to float 57 -> 41; 1024^3 13.5 -> 10.2.
+ *
  * ROWS: the scale of A differs between the rows of a wave (blockA = 1): a multiplication more per element and slab.
  *
  * A wave that multiplies goes before one that loads, stores or waits on the same SIMD, and the loads are issued in the first
@@ -84,7 +88,7 @@ template <bool KC, int R> static __device__ __forceinline__ och_u32x4 f8_any_chu
    return f8_border_chunk(mat + (KC ? gk + gr * ld : gr + gk * ld), valid, KC ? K : rows);
 }
 
-/* The chunks that a thread moves: threadIdx.x + THREADS i of every slab. They differ by whole rows (KC) or whole k (!KC)
+/* The chunks that thread t of THREADS moves: t + THREADS i of every slab. They differ by whole rows (KC) or whole k (!KC)
    with the same twist. Rows that do not exist are never loaded: KC repeats the last row instead; !KC loads the last 16
    rows where a chunk passes the end, and moves them into place on the way to LDS (so `rows` is at least 16 there). What
    these lanes hold for rows outside the matrix reaches only elements of C that are not written. */
@@ -101,7 +105,7 @@ template <bool KC, int R, int THREADS> struct F8Stage
    static __device__ __forceinline__ bool pipelined(uint32_t rows, int64_t ld) { return (KC || rows >= 16) && ld < (1 << 24); }
    __device__ __forceinline__ void start(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows)
    {  uint32_t row, k;
-      L::where(threadIdx.x, row, k);
+      L::where(threadIdx.x % THREADS, row, k);
       slab = mat + (KC ? (int64_t)k0 + (int64_t)r0 * ld : (int64_t)r0 + (int64_t)k0 * ld);
       const uint32_t last = rows - r0 < R ? rows - r0 - 1 : R - 1;        /* the tile's last row */
       move = 0;
@@ -127,7 +131,7 @@ template <bool KC, int R, int THREADS> struct F8Stage
    /* any slab, chunk by chunk */
    __device__ __forceinline__ void load_border(const uint8_t *mat, int64_t ld, uint32_t r0, uint32_t k0, uint32_t rows, uint32_t K)
    {  move = 0;
-      uint32_t thread = threadIdx.x;
+      uint32_t thread = threadIdx.x % THREADS;
       asm volatile("" : "+v"(thread));   /* what follows from it is computed here, not kept in registers through the pipelined slabs */
 #pragma unroll
       for (int i = 0; i < NV; i++) v[i] = f8_any_chunk<KC, R>(mat, ld, r0, k0, rows, K, thread + THREADS * i);
@@ -137,7 +141,7 @@ template <bool KC, int R, int THREADS> struct F8Stage
 #pragma unroll
       for (int i = 0; i < NV; i++)
       {  if (!KC && border) v[i] = f8_shift(v[i], move);
-         *reinterpret_cast<och_u32x4 *>(slab + 16 * (threadIdx.x + THREADS * i)) = v[i];
+         *reinterpret_cast<och_u32x4 *>(slab + 16 * (threadIdx.x % THREADS + THREADS * i)) = v[i];
       }
    }
 };
@@ -193,15 +197,17 @@ template <int DT, int R, uint32_t PITCH, uint32_t COLUMNS, int THREADS> __device
    }
 }
 
-template <bool AKC, bool BKC, bool E5A, bool E5B, bool WIDE, bool ROWS>
-__global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(const F8GemmParams p)
+template <bool AKC, bool BKC, bool E5A, bool E5B, bool WIDE, bool ROWS, bool PAIR>
+__global__ __launch_bounds__(OCH_F8_TILE_THREADS * (PAIR ? 2 : 1), 2) void gemm_f8_tile_kernel(const F8GemmParams p)
 {
    constexpr int R = OCH_F8_TILE, THREADS = OCH_F8_TILE_THREADS, OPERAND = R * OCH_F8_SLAB, BUF = 2 * OPERAND + 2 * R * 4;
-   __shared__ __align__(16) char lds[2 * BUF];
+   __shared__ __align__(16) char all_lds[(PAIR ? 4 : 2) * BUF];
+   const uint32_t thread = threadIdx.x % THREADS, group = PAIR ? __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS) : 0;
+   char *const lds = all_lds + group * (2 * BUF);
    uint32_t tm, tn;
    f8_tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
    const uint32_t m0 = tm * R, n0 = tn * R;
-   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % 2 * 64, wn = wave / 2 * 64;
+   const uint32_t lane = threadIdx.x & 63, wave = thread >> 6, wm = wave % 2 * 64, wn = wave / 2 * 64;
    const och_f32x4v zero = { 0, 0, 0, 0 };
    och_f32x4v acc[4][4];
 #pragma unroll
@@ -212,10 +218,15 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
    const uint32_t all = (p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB;
    uint32_t s = 0, end = all;
    if (p.share_slabs) { s = blockIdx.y * p.share_slabs; end = s + p.share_slabs < all ? s + p.share_slabs : all; }
+   uint32_t turns = end - s;
+   if (PAIR)
+   {  turns = (turns + 1) / 2;
+      if (group == 0) end = s + turns; else s += turns;      /* the second group may have one slab less */
+   }
 
    /* every thread brings one scale: waves 0 and 1 of A's rows, 2 and 3 of B's columns; those outside C repeat the last */
    const bool forA = __builtin_amdgcn_readfirstlane(wave) < 2;
-   const uint32_t line = threadIdx.x % R, most = (forA ? p.M - m0 : p.N - n0) - 1, shift = forA ? p.shiftA : p.shiftB, begin = forA ? m0 : n0;
+   const uint32_t line = thread % R, most = (forA ? p.M - m0 : p.N - n0) - 1, shift = forA ? p.shiftA : p.shiftB, begin = forA ? m0 : n0;
    const uint32_t scale_of = ((begin + (line < most ? line : most)) >> shift) - (begin >> shift);
    const int64_t scale_line = forA ? p.sa_m : p.sb_n, scale_step = forA ? p.sa_k : p.sb_k;
    const float *scale = (forA ? p.SA : p.SB) + (int64_t)(begin >> shift) * scale_line + (int64_t)s * scale_step;
@@ -223,23 +234,24 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
 
    /* slabs that are whole along k are pipelined; the rest of K, and everything of an operand of under 16 contiguous rows or
       of columns 16 MB apart, is not */
-   const uint32_t whole = p.K / OCH_F8_SLAB, piped = !F8Stage<AKC, R, THREADS>::pipelined(p.M, p.ldA) || !F8Stage<BKC, R, THREADS>::pipelined(p.N, p.ldB) ? s : end < whole ? end : whole;
+   const uint32_t whole = p.K / OCH_F8_SLAB, piped = PAIR ? end : !F8Stage<AKC, R, THREADS>::pipelined(p.M, p.ldA) || !F8Stage<BKC, R, THREADS>::pipelined(p.N, p.ldB) ? s : end < whole ? end : whole;
    const bool borderA = m0 + R > p.M, borderB = n0 + R > p.N;
    F8Stage<AKC, R, THREADS> la; F8Stage<BKC, R, THREADS> lb; float ls = 0;
    la.start(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M); lb.start(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N);
    auto stash = [&](char *buf)
    {  la.store(buf, borderA); lb.store(buf + OPERAND, borderB);
-      reinterpret_cast<float *>(buf + 2 * OPERAND)[threadIdx.x] = ls;
+      reinterpret_cast<float *>(buf + 2 * OPERAND)[thread] = ls;
    };
    if (s < piped)
    {  la.load(p.ldA); lb.load(p.ldB); ls = next_scale();
       stash(lds);
    }
    __syncthreads();
-   for (uint32_t turn = 0; s < end; s++, turn ^= 1)
-   {  char *buf = lds + turn * BUF;
+   for (uint32_t turn = 0; turns > 0; turns--, s++, turn ^= 1)
+   {  if (PAIR && s >= end) { __syncthreads(); continue; }
+      char *buf = lds + turn * BUF;
       const float *sA = reinterpret_cast<const float *>(buf + 2 * OPERAND), *sB = sA + R;
-      if (s >= piped)
+      if (!PAIR && s >= piped)
       {  la.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); lb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); ls = next_scale();
          stash(buf);
          __syncthreads();
@@ -302,38 +314,53 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS, 2) void gemm_f8_tile_kernel(co
    /* the tile leaves through LDS, where the slabs were; a share of K as raw sums into the share's plane */
    constexpr uint32_t PITCH = R * 4 + 16;
    static_assert(R * PITCH <= 2 * BUF, "the tile fits where the slabs were");
-   {  char *mine = lds + (wn + lane % 16) * PITCH + (wm + 4 * (lane / 16)) * 4;
+   char *const mine = lds + (wn + lane % 16) * PITCH + (wm + 4 * (lane / 16)) * 4;
+   auto put = [&]()
+   {
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
          for (int i = 0; i < 4; i++) *reinterpret_cast<och_f32x4v *>(mine + 16 * j * PITCH + 64 * i) = acc[i][j];
+   };
+   if (PAIR)
+   {  if (group == 1) put();
+      __syncthreads();
+      if (group == 0)
+      {
+#pragma unroll
+         for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i][j] += *reinterpret_cast<const och_f32x4v *>(mine + 2 * BUF + 16 * j * PITCH + 64 * i);
+      }
    }
+   if (group == 0) put();
    __syncthreads();
    if (p.share_slabs)
    {  F8GemmParams q = p;
       q.ldC = f8_plane_pitch(p.M); q.C = reinterpret_cast<char *>(p.partial + (size_t)blockIdx.y * q.ldC * p.N); q.alpha = 1.0f; q.beta = 0.0f;
-      f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS>(q, lds, m0, n0);
+      f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS * (PAIR ? 2 : 1)>(q, all_lds, m0, n0);
    }
-   else if (WIDE)                 f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS>(p, lds, m0, n0);
-   else if (p.dtypeC == OCH_HALF) f8_store_columns<OCH_HALF, R, PITCH, R, THREADS>(p, lds, m0, n0);
-   else                           f8_store_columns<OCH_BFLOAT16, R, PITCH, R, THREADS>(p, lds, m0, n0);
+   else if (WIDE)                 f8_store_columns<OCH_FLOAT, R, PITCH, R, THREADS * (PAIR ? 2 : 1)>(p, all_lds, m0, n0);
+   else if (p.dtypeC == OCH_HALF) f8_store_columns<OCH_HALF, R, PITCH, R, THREADS * (PAIR ? 2 : 1)>(p, all_lds, m0, n0);
+   else                           f8_store_columns<OCH_BFLOAT16, R, PITCH, R, THREADS * (PAIR ? 2 : 1)>(p, all_lds, m0, n0);
 }
 
-template <bool E5A, bool E5B, bool WIDE, bool ROWS> static int gemm_f8_tile_launch(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream)
+template <bool E5A, bool E5B, bool WIDE, bool ROWS, bool PAIR> static int gemm_f8_tile_launch(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream)
 {
-   const dim3 block(OCH_F8_TILE_THREADS);
-   if (akc && bkc) hipLaunchKernelGGL((gemm_f8_tile_kernel<true, true, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
-   else if (akc)   hipLaunchKernelGGL((gemm_f8_tile_kernel<true, false, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
-   else if (bkc)   hipLaunchKernelGGL((gemm_f8_tile_kernel<false, true, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
-   else            hipLaunchKernelGGL((gemm_f8_tile_kernel<false, false, E5A, E5B, WIDE, ROWS>), grid, block, 0, stream, p);
+   const dim3 block(OCH_F8_TILE_THREADS * (PAIR ? 2 : 1));
+   if (akc && bkc) hipLaunchKernelGGL((gemm_f8_tile_kernel<true, true, E5A, E5B, WIDE, ROWS, PAIR>), grid, block, 0, stream, p);
+   else if (akc)   hipLaunchKernelGGL((gemm_f8_tile_kernel<true, false, E5A, E5B, WIDE, ROWS, PAIR>), grid, block, 0, stream, p);
+   else if (bkc)   hipLaunchKernelGGL((gemm_f8_tile_kernel<false, true, E5A, E5B, WIDE, ROWS, PAIR>), grid, block, 0, stream, p);
+   else            hipLaunchKernelGGL((gemm_f8_tile_kernel<false, false, E5A, E5B, WIDE, ROWS, PAIR>), grid, block, 0, stream, p);
    OCH_CHECK_LAUNCH();
    return 0;
 }
-template <bool E5A, bool E5B> static int gemm_f8_tile(const F8GemmParams &p, bool akc, bool bkc, dim3 grid, hipStream_t stream)
+template <bool E5A, bool E5B> static int gemm_f8_tile(const F8GemmParams &p, bool akc, bool bkc, bool pair, dim3 grid, hipStream_t stream)
 {
    const bool wide = p.dtypeC == OCH_FLOAT, rows = p.shiftA == 0;
-   return wide ? (rows ? gemm_f8_tile_launch<E5A, E5B, true, true>(p, akc, bkc, grid, stream) : gemm_f8_tile_launch<E5A, E5B, true, false>(p, akc, bkc, grid, stream))
-               : (rows ? gemm_f8_tile_launch<E5A, E5B, false, true>(p, akc, bkc, grid, stream) : gemm_f8_tile_launch<E5A, E5B, false, false>(p, akc, bkc, grid, stream));
+#define OCH_GO(WIDE, ROWS) (pair ? gemm_f8_tile_launch<E5A, E5B, WIDE, ROWS, true>(p, akc, bkc, grid, stream) : gemm_f8_tile_launch<E5A, E5B, WIDE, ROWS, false>(p, akc, bkc, grid, stream))
+   return wide ? (rows ? OCH_GO(true, true) : OCH_GO(true, false)) : (rows ? OCH_GO(false, true) : OCH_GO(false, false));
+#undef OCH_GO
 }
 
 } /* namespace och */

@@ -509,3 +509,18 @@ def test_gemm_large(hip, stream, ta, tb, ba, bb):
         bv = (F.decode(b, F.E4M3) * wide_scales(sb, bb, N, K)).astype(np.float32)
         want = F.from_wide(F.to_wide(bv @ av.T, F.BF16), F.BF16)        # whole multiples of 1/4 below 2^22: exact in float
         assert np.array_equal(got, want), (M, N, K, np.argwhere(got != want)[:5])
+
+
+@pytest.mark.parametrize("dtype", [F.FLOAT, F.BF16], ids=name_of)
+@pytest.mark.parametrize("ba", [1, 128])
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_gemm_exact_with_halves_of_k(hip, stream, ta, tb, ba, dtype):
+    """K of whole blocks, odd numbers of them too, where two groups of waves share a tile, alone and with shares of K whose
+    last is shorter. (Sums stay below 2^6 K 2^2 < 2^21: exact in float.)"""
+    rng = np.random.default_rng(ba + ord(tb))
+    for M, N, K, pad in [(640, 640, 896, 0), (1024, 1024, 1152, 16), (130, 140, 896, 3), (2048, 130, 4224, 0), (300, 1000, 2688, 5), (1500, 1400, 256, 0), (256, 384, 8064, 1)]:
+        a, sa, b, sb = exact_case(rng, M, N, K, ba, 1)
+        got = run_gemm(stream, F.E4M3, F.E4M3, dtype, ta, tb, a, sa, ba, b, sb, 1, pad=(pad, pad, pad), shift=(pad, pad, pad))
+        av, bv = F.decode(a, F.E4M3) * wide_scales(sa, ba, M, K), F.decode(b, F.E4M3) * wide_scales(sb, 1, N, K)
+        want = (bv.astype(np.float32) @ av.astype(np.float32).T)
+        assert np.array_equal(got, F.to_wide(want, dtype)), (M, N, K)
