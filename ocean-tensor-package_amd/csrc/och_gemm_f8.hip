@@ -38,7 +38,7 @@ template <int DT> __global__ __launch_bounds__(256) void gemm_f8_join_kernel(con
    16.0, twenty 14.4, forty 16.8. Pairs of groups on a tile work like two workgroups on a unit and need no plane of their own.
    Blocks per share at the least of blocks * slab + blocks of K / blocks * plane, and the numbers of shares that fill every unit
    once and twice, are compared with one. */
-static uint64_t gemm_f8_shares(uint64_t tiles, uint64_t slabs, uint64_t plane_bytes, uint64_t units, bool wide, bool piped, bool can_pair, bool *pair)
+static uint64_t gemm_f8_shares(uint64_t tiles, uint64_t slabs, uint64_t plane_bytes, uint64_t units, bool wide, bool piped, bool *pair)
 {
    uint64_t best = 1, most = 2 * units / tiles;
    const uint64_t fit = OCH_GEMM_WORKSPACE / plane_bytes;
@@ -50,12 +50,13 @@ static uint64_t gemm_f8_shares(uint64_t tiles, uint64_t slabs, uint64_t plane_by
    double least = INFINITY;
    *pair = false;
    for (int i = 0; i < 6; i++)
-   {  const uint64_t s = tries[i] < most ? tries[i] : most, own = s < 2 ? slabs : (slabs + s - 1) / s;
-      if (s < 2 && i > 0) continue;
-      const double join = s < 2 ? 0 : 4.0 + (double)s * plane;
+   {  uint64_t s = tries[i] < most ? tries[i] : most;
+      if (s < 1) s = 1;
+      const uint64_t own = (slabs + s - 1) / s;
+      const double join = s > 1 ? 4.0 + (double)s * plane : 0;
       const double single = (double)own * slab * (tiles * s > units ? 1.5 : 1.0) + join, twin = (double)((own + 1) / 2) * slab * 1.5 + 0.5 + join;
-      if (single < least) { least = single; best = s < 2 ? 1 : s; *pair = false; }
-      if (can_pair && own > 1 && tiles * s <= units && twin < least) { least = twin; best = s < 2 ? 1 : s; *pair = true; }
+      if (single < least) { least = single; best = s; *pair = false; }
+      if (piped && own > 1 && tiles * s <= units && twin < least) { least = twin; best = s; *pair = true; }
    }
    return best;
 }
@@ -68,7 +69,7 @@ static int gemm_f8_tiles(F8GemmParams p, bool e5a, bool e5b, bool akc, bool bkc,
    if (tiles > most_groups(OCH_F8_TILE_THREADS)) return set_error("gemm_scaled: a result of %u x %u has too many tiles", p.M, p.N);
    const bool piped = (akc || p.M >= 16) && (bkc || p.N >= 16) && p.ldA < (1 << 24) && p.ldB < (1 << 24);
    bool pair;
-   uint64_t shares = gemm_f8_shares(tiles, slabs, (uint64_t)f8_plane_pitch(p.M) * p.N * sizeof(float), units, p.dtypeC == OCH_FLOAT, piped, piped && p.K % OCH_F8_SLAB == 0, &pair);
+   uint64_t shares = gemm_f8_shares(tiles, slabs, (uint64_t)f8_plane_pitch(p.M) * p.N * sizeof(float), units, p.dtypeC == OCH_FLOAT, piped, &pair);
    if (shares >= 2)
    {  char *ws;
       if (stream_gemm_workspace(stream, &ws) != 0) return -1;

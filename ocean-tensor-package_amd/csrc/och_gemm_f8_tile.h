@@ -6,8 +6,8 @@
  * alignment; at the matrix's border they are put together from two that overlap.
  *
  * PAIR: where there are no more tiles than compute units, two groups of four waves share a tile, each with its half of K and
- * LDS of its own, as two workgroups would; their sums meet in LDS. Only for K of whole slabs, all pipelined: the groups have
- * one barrier in common. 2048 x 2048 x 4096 to bfloat16 40 -> 28.5 us, to float 57 -> 41; 1024^3 13.5 -> 10.2.
+ * LDS of its own, as two workgroups would; their sums meet in LDS. The groups have their barriers in common, which is why every
+ * slab but the last of K has to be pipelined. 2048 x 2048 x 4096 to bfloat16 40 -> 28.5 us, to float 57 -> 41; 1024^3 13.5 -> 10.2.
  *
  * ROWS: the scale of A differs between the rows of a wave (blockA = 1): a multiplication more per element and slab.
  *
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS * (PAIR ? 2 : 1), 2) void gemm_
    uint32_t tm, tn;
    f8_tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
    const uint32_t m0 = tm * R, n0 = tn * R;
-   const uint32_t lane = threadIdx.x & 63, wave = thread >> 6, wm = wave % 2 * 64, wn = wave / 2 * 64;
+   const uint32_t lane = threadIdx.x & 63, wave = PAIR ? __builtin_amdgcn_readfirstlane(thread >> 6) : thread >> 6, wm = wave % 2 * 64, wn = wave / 2 * 64;
    const och_f32x4v zero = { 0, 0, 0, 0 };
    och_f32x4v acc[4][4];
 #pragma unroll
@@ -218,10 +218,13 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS * (PAIR ? 2 : 1), 2) void gemm_
    const uint32_t all = (p.K + OCH_F8_SLAB - 1) / OCH_F8_SLAB;
    uint32_t s = 0, end = all;
    if (p.share_slabs) { s = blockIdx.y * p.share_slabs; end = s + p.share_slabs < all ? s + p.share_slabs : all; }
-   uint32_t turns = end - s;
+   const uint32_t whole = p.K / OCH_F8_SLAB;
+   uint32_t turns = end - s, rest = ~0u;                     /* rest: the turn in which one of the groups takes the slab inside which K ends */
    if (PAIR)
-   {  turns = (turns + 1) / 2;
-      if (group == 0) end = s + turns; else s += turns;      /* the second group may have one slab less */
+   {  const uint32_t half = (turns + 1) / 2, second = s + half;
+      if (end > whole) rest = whole - (end > second ? second : s);
+      if (group == 0) end = second; else s = second;         /* the second group may have one slab less */
+      turns = half;
    }
 
    /* every thread brings one scale: waves 0 and 1 of A's rows, 2 and 3 of B's columns; those outside C repeat the last */
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS * (PAIR ? 2 : 1), 2) void gemm_
 
    /* slabs that are whole along k are pipelined; the rest of K, and everything of an operand of under 16 contiguous rows or
       of columns 16 MB apart, is not */
-   const uint32_t whole = p.K / OCH_F8_SLAB, piped = PAIR ? end : !F8Stage<AKC, R, THREADS>::pipelined(p.M, p.ldA) || !F8Stage<BKC, R, THREADS>::pipelined(p.N, p.ldB) ? s : end < whole ? end : whole;
+   const uint32_t piped = !F8Stage<AKC, R, THREADS>::pipelined(p.M, p.ldA) || !F8Stage<BKC, R, THREADS>::pipelined(p.N, p.ldB) ? s : end < whole ? end : whole;
    const bool borderA = m0 + R > p.M, borderB = n0 + R > p.N;
    F8Stage<AKC, R, THREADS> la; F8Stage<BKC, R, THREADS> lb; float ls = 0;
    la.start(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M); lb.start(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N);
@@ -247,15 +250,18 @@ __global__ __launch_bounds__(OCH_F8_TILE_THREADS * (PAIR ? 2 : 1), 2) void gemm_
       stash(lds);
    }
    __syncthreads();
-   for (uint32_t turn = 0; turns > 0; turns--, s++, turn ^= 1)
-   {  if (PAIR && s >= end) { __syncthreads(); continue; }
+   for (uint32_t round = 0; round < turns; round++, s++)
+   {  const uint32_t turn = round & 1;
       char *buf = lds + turn * BUF;
       const float *sA = reinterpret_cast<const float *>(buf + 2 * OPERAND), *sB = sA + R;
-      if (!PAIR && s >= piped)
-      {  la.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); lb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); ls = next_scale();
-         stash(buf);
+      if (PAIR ? round == rest : s >= piped)
+      {  if (!PAIR || (s >= piped && s < end))
+         {  la.load_border(p.A, p.ldA, m0, s * OCH_F8_SLAB, p.M, p.K); lb.load_border(p.B, p.ldB, n0, s * OCH_F8_SLAB, p.N, p.K); ls = next_scale();
+            stash(buf);
+         }
          __syncthreads();
       }
+      if (PAIR && s >= end) { __syncthreads(); continue; }
       const bool more = s + 1 < piped;
       F8Operand<WIDE> b[4]; float t[4];
       {  och_i32x8 c[4];

@@ -515,10 +515,11 @@ def test_gemm_large(hip, stream, ta, tb, ba, bb):
 @pytest.mark.parametrize("ba", [1, 128])
 @pytest.mark.parametrize("ta,tb", TRANS)
 def test_gemm_exact_with_halves_of_k(hip, stream, ta, tb, ba, dtype):
-    """K of whole blocks, odd numbers of them too, where two groups of waves share a tile, alone and with shares of K whose
-    last is shorter. (Sums stay below 2^6 K 2^2 < 2^21: exact in float.)"""
+    """Where two groups of waves share a tile: even and odd numbers of blocks, K that ends inside one, shares of K whose last is
+    shorter. (Sums stay below 2^6 K 2^2 < 2^21: exact in float.)"""
     rng = np.random.default_rng(ba + ord(tb))
-    for M, N, K, pad in [(640, 640, 896, 0), (1024, 1024, 1152, 16), (130, 140, 896, 3), (2048, 130, 4224, 0), (300, 1000, 2688, 5), (1500, 1400, 256, 0), (256, 384, 8064, 1)]:
+    for M, N, K, pad in [(640, 640, 896, 0), (1024, 1024, 1152, 16), (130, 140, 896, 3), (2048, 130, 4224, 0), (300, 1000, 2688, 5), (1500, 1400, 256, 0), (256, 384, 8064, 1), (700, 700, 1000, 4),
+                         (1024, 700, 1030, 0), (2000, 1900, 130, 0), (300, 200, 4001, 1), (130, 900, 8200, 8)]:
         a, sa, b, sb = exact_case(rng, M, N, K, ba, 1)
         got = run_gemm(stream, F.E4M3, F.E4M3, dtype, ta, tb, a, sa, ba, b, sb, 1, pad=(pad, pad, pad), shift=(pad, pad, pad))
         av, bv = F.decode(a, F.E4M3) * wide_scales(sa, ba, M, K), F.decode(b, F.E4M3) * wide_scales(sb, 1, N, K)
