@@ -124,12 +124,19 @@ int och_device_synchronize(void);
 int och_stream_create(och_stream *stream);                 /* device_gpu.c:251-288 */
 int och_stream_destroy(och_stream stream);                 /* device_gpu.c:324-346 */
 int och_stream_synchronize(och_stream stream);             /* device_gpu.c:374-382 */
-/* No counterpart in the reference. Products that are cut along K, matrix-vector products and sliced axis reductions  */
-/* keep partial results in a 64 MB workspace that belongs to the stream (taken from the stream-ordered pool at the     */
-/* first such call, or by och_stream_begin_capture; released with the stream). A caller that retires a stream without */
-/* destroying it -- Ocean's device layer recycles up to 64 of them -- gives the workspace back with this call; it is   */
-/* freed behind the work already queued on the stream and the next call that needs one takes a new one. A graph         */
-/* recorded on the stream addresses the old workspace and must not be launched after this call.                        */
+/* No counterpart in the reference. Products that are cut along K, matrix-vector products, sliced axis reductions and  */
+/* the norm's gradient of the weights keep partial results in a 64 MB workspace that belongs to the stream (taken from */
+/* the stream-ordered pool at the first such call, or by och_stream_begin_capture; released with the stream). A caller */
+/* that retires a stream without destroying it -- Ocean's device layer recycles up to 64 of them -- gives the          */
+/* workspace back with release_workspace; it is freed behind the work already queued on the stream and the next call   */
+/* that needs one takes a new one. A graph recorded on the stream addresses the old workspace and must not be launched */
+/* after this call; while the stream records, the call is an error. These calls launch several kernels in a row:       */
+/* host threads that share a stream take turns.                                                                        */
+/* reserve_workspace creates the workspace and the reductions' scratch without any other work. A program that records  */
+/* with another library's graphs, so not through och_stream_begin_capture, calls it before it begins: a call that      */
+/* finds no workspace while its stream records is an error. Such a graph, too, is launched on the stream that recorded */
+/* it and on no other.                                                                                                 */
+int och_stream_reserve_workspace(och_stream stream);
 int och_stream_release_workspace(och_stream stream);
 int och_stream_wait_event(och_stream stream, och_event event); /* device_gpu.c:411-420 */
 int och_event_create(och_event *event, int timing);        /* device_gpu.c:292-320; timing=0: disable timing */
@@ -422,7 +429,9 @@ int och_mgs_project(int dtype, size_t n, size_t k, const void *Q, ptrdiff_t ldq,
 /* Pointers are aligned to their element; sizes, leading dimensions and     */
 /* starts may be odd (whole 16-byte units are only faster). Matrices of one */
 /* call must not overlap unless stated. No call synchronises or allocates   */
-/* beyond the stream's workspace, so all can be recorded into a graph.      */
+/* beyond the stream's workspace, so all can be recorded into a graph (by   */
+/* other means than och_stream_begin_capture: behind                        */
+/* och_stream_reserve_workspace).                                           */
 /* ======================================================================== */
 enum { OCH_BFLOAT16 = 32, OCH_FLOAT8_E4M3 = 33, OCH_FLOAT8_E5M2 = 34 };     /* e4m3: largest value 448, no infinity; e5m2: 57344 */
 

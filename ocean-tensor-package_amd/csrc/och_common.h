@@ -49,7 +49,7 @@ int fill_bytes(void *dst, int value, size_t nbytes, hipStream_t stream);
 
 /* Scratch memory that kernels of one stream share: work on one stream is ordered, work on different streams is not
    (Ocean gives every storage its own stream), so every (device, stream) pair owns its scratch. It is created on the
-   first use of the stream -- or by och_device_warmup / och_stream_begin_capture, so that no allocation happens while
+   first use of the stream -- or by och_device_warmup / och_stream_reserve_workspace / och_stream_begin_capture, so that no allocation happens while
    a stream records -- and released when the stream is destroyed. */
 #define OCH_RED_MAX_BLOCKS 512
 #define OCH_RED_SLOT 16                               /* bytes per partial of a full reduction */

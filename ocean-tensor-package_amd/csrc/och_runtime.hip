@@ -30,6 +30,14 @@ namespace och {
 static std::map<std::pair<int, hipStream_t>, StreamContext> g_stream_ctx;
 static std::mutex g_stream_ctx_mutex;
 
+/* whether the stream records a graph (the default stream cannot) */
+static int stream_records(hipStream_t stream, bool *records)
+{
+   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+   if (stream != nullptr) OCH_CHECK_HIP(hipStreamIsCapturing(stream, &capturing));
+   *records = capturing != hipStreamCaptureStatusNone;
+   return 0;
+}
 int stream_context(hipStream_t stream, StreamContext **out)
 {
    int dev;
@@ -42,10 +50,9 @@ int stream_context(hipStream_t stream, StreamContext **out)
       void *scratch = nullptr, *host = nullptr;
       /* the scratch cannot be created while the stream records a graph: allocation is not a graph node, and the
          zeroing below would become one and run again at every replay, in the middle of the recorded reductions */
-      hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-      if (stream != nullptr) OCH_CHECK_HIP(hipStreamIsCapturing(stream, &capturing));
-      if (capturing != hipStreamCaptureStatusNone)
-         return set_error("a stream must be used once, or recording must start with och_stream_begin_capture, before library calls are recorded on it");
+      bool records;
+      if (stream_records(stream, &records) != 0) return -1;
+      if (records) return set_error("a stream needs its scratch before library calls are recorded on it: och_stream_reserve_workspace, or recording begins with och_stream_begin_capture");
       OCH_CHECK_HIP(hipMalloc(&scratch, OCH_RED_SCRATCH));
       /* zeroed by a kernel on the owning stream itself: ordered before the stream's first reduction by the stream,
          whatever its blocking mode with respect to the null stream */
@@ -64,7 +71,11 @@ int stream_gemm_workspace(hipStream_t stream, char **workspace)
    if (stream_context(stream, &c) != 0) return -1;
    std::lock_guard<std::mutex> lock(g_stream_ctx_mutex);
    if (c->gemm_workspace == nullptr)
-   {  /* from the stream-ordered pool: no device-wide synchronisation, and what och_stream_release_workspace gives back
+   {  /* what is allocated while the stream records belongs to the recorded graph: later calls may not write to it */
+      bool records;
+      if (stream_records(stream, &records) != 0) return -1;
+      if (records) return set_error("a stream needs its workspace before this call is recorded on it: och_stream_reserve_workspace, or recording begins with och_stream_begin_capture");
+      /* from the stream-ordered pool: no device-wide synchronisation, and what och_stream_release_workspace gives back
          serves the next stream that needs one */
       void *w = nullptr;
       OCH_CHECK_HIP(hipMallocAsync(&w, OCH_GEMM_WORKSPACE, stream));
@@ -81,6 +92,9 @@ int stream_release_workspace(hipStream_t stream)
    std::lock_guard<std::mutex> lock(g_stream_ctx_mutex);
    auto it = g_stream_ctx.find(std::make_pair(dev, stream));
    if (it == g_stream_ctx.end() || it->second.gemm_workspace == nullptr) return 0;
+   bool records;
+   if (stream_records(stream, &records) != 0) return -1;
+   if (records) return set_error("a stream that records a graph keeps its workspace");
    char *w = it->second.gemm_workspace;
    it->second.gemm_workspace = nullptr;
    OCH_CHECK_HIP(hipFreeAsync(w, stream));
@@ -226,6 +240,7 @@ int och_stream_destroy(och_stream stream)
    OCH_CHECK_HIP(hipStreamDestroy((hipStream_t)stream));
    return 0;
 }
+int och_stream_reserve_workspace(och_stream stream) { char *workspace; return och::stream_gemm_workspace((hipStream_t)stream, &workspace); }
 int och_stream_release_workspace(och_stream stream) { return och::stream_release_workspace((hipStream_t)stream); }
 int och_stream_synchronize(och_stream stream) { OCH_CHECK_HIP(hipStreamSynchronize((hipStream_t)stream)); OCH_CHECK_AFTER_WAIT("a stream"); return 0; }
 int och_stream_wait_event(och_stream stream, och_event event)
