@@ -471,6 +471,11 @@ int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *dY, ptrdiff_
 /* A float result has sums as good as float additions make them. For half and bfloat16 results the 8-bit matrix            */
 /* instruction adds eight products at a time and cuts off what lies below 2^-13 of the largest of them: about 1e-4 of the  */
 /* result's norm on Gaussian operands, less than the rounding to half.                                                     */
+/* The two scales of a block are multiplied with each other first, in float, and their product with the block's sum: it    */
+/* has to be finite, or every result that the block takes part in is infinite or NaN, and at 2^-126 or more for the block  */
+/* to count in full (from 2^-149 down it counts as nothing). Two scales between 2^-63 and 2^63, those of blocks whose      */
+/* largest magnitudes lie between 2^-47 and 2^71, always are; a block of zeros, whose scale is 2^-100 / c, needs a finite  */
+/* product only.                                                                                                           */
 /* beta = 0 does not read C; K = 0 leaves beta * C. Sums are added in an order that depends on sizes, types, leading        */
 /* dimensions, alignment and the device alone: results are reproducible.                                                   */
 int och_gemm_scaled(int dtypeA, int dtypeB, int dtypeC, char transA, char transB, size_t M, size_t N, size_t K, float alpha,

@@ -4,6 +4,10 @@
  * The matrix cores multiply a whole block of 128 k (one v_mfma_f32_16x16x128_f8f6f4, or four bfloat16 ones where the
  * result is float); the 16 x 16 sums of a block are multiplied by the two scales and added to the float accumulators
  * outside them, four multiply-adds per lane beside 32 or 64 cycles of matrix work.
+ *
+ * The two scales are multiplied with each other first, which is once per column and block where a scale of A covers 128
+ * rows; either one times the sums would be once more per element. So their product has to lie within float's range, and
+ * callers are told so; sums times a single scale would leave the range for other pairs (1e35 times a sum of 1e7).
  */
 #include "och_gemm_f8_tile.h"
 #include <math.h>

@@ -902,7 +902,8 @@ def rmsNormGradient(dy, h, rstd, weight=None, dsum=None):
 
 def gemmScaled(alpha, a, sa, b, sb, beta=0.0, c=None, transA="N", transB="N", codeA="e4m3", codeB="e4m3", dt=float):
     """alpha op(A) op(B) + beta C of two matrices in 8-bit codes with their scales, as quantizeBlocks and rmsNorm make them;
-    C is written if given, or a new matrix of type dt (half or float)."""
+    C is written if given, or a new matrix of type dt (half or float). The product of the two scales of a block has to be a
+    finite float, and at least 2^-126 for the block to count in full."""
     if c is None:
         if beta != 0:
             raise ValueError("gemmScaled: beta without C")
