@@ -62,9 +62,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantizeParams
 /* Blocks of 1 x 128 and 128 x 128 (WHOLE): a workgroup of 256 owns 128 x 128 elements; thread t holds rows
    8 (t % 16) .. + 7 of columns t / 16 + 16 c, c = 0 .. 7. The maxima over the columns are taken in registers first, then
    over the four groups of lanes of the wave, and then the four waves' meet in LDS.
-   8192 x 4096 floats in 128 x 128 blocks: 30.0 us (5.6 TB/s), 31.6 where all sixteen threads of a column meet in LDS;
-   5003 x 4001 halfs, too few for a second round of workgroups, in 1 x 128 blocks: 17.2 us (3.5 TB/s) against 19.6, with 64 rows
-   to a workgroup 20.2. */
+   8192 x 4096 floats in 128 x 128 blocks: 29.6 us (5.7 TB/s), 31.6 where all sixteen threads of a column meet in LDS.
+   Halfs in 1 x 128 blocks: 5120 x 4096, columns of whole cache lines, 11.4 us (5.6 TB/s); 5003 x 4001 17.3 us (3.5 TB/s), with 64
+   rows to a workgroup 20.2: neighbouring tiles share lines and run on different dies, so that 39 % more is read and 21 % more
+   written than the matrix holds. */
 template <int DT, int CODE, bool WHOLE, bool NT>
 __global__ __launch_bounds__(256) void quantize_tile_kernel(const QuantizeParams p)
 {
