@@ -53,7 +53,8 @@ typedef __bf16 och_bf16x8 __attribute__((ext_vector_type(8)));
  * eights, and in the older fp8 instructions alike, 24 bits do). On Gaussian operands that is about 1e-4 of the result's
  * norm: half a rounding to half, a twentieth of one to bfloat16.
  * WIDE: the codes become bfloat16, which holds them exactly, and four v_mfma_f32_16x16x32_bf16 of 16 cycles add their
- * exact products with 24 bits: sums as good as float ones, for results that are float, at half the matrix rate. */
+ * exact products with 24 bits: sums as good as float ones, at half the matrix rate, for results that are float and wherever
+ * memory bounds the product anyway (the kernel of few columns, up to 32 of them). */
 template <bool WIDE> struct F8Operand;
 template <> struct F8Operand<false>
 {  och_i32x8 v;

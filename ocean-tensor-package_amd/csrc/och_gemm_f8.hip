@@ -2,7 +2,7 @@
  * operand. No counterpart in the reference.
  *
  * The matrix cores multiply a whole block of 128 k (one v_mfma_f32_16x16x128_f8f6f4, or four bfloat16 ones where the
- * result is float); the 16 x 16 sums of a block are multiplied by the two scales and added to the float accumulators
+ * result is float or has up to 32 columns); the 16 x 16 sums of a block are multiplied by the two scales and added to the float accumulators
  * outside them, four multiply-adds per lane beside 32 or 64 cycles of matrix work.
  *
  * The two scales are multiplied with each other first, which is once per column and block where a scale of A covers 128

@@ -11,8 +11,8 @@
  * end, where the waves' sums meet in LDS and are added in the order of the waves. Two tiles of rows share the columns' codes
  * where there are more than 16 columns and rows enough: these come from the second-level cache once per workgroup and slab.
  *
- * Measured, three sets of operands in turn: 14336 x 1 x 4096 10.9 us (5.4 TB/s), 8192 x 16 x 8192 11.9 us (5.7 TB/s), 8192 x
- * 48 x 8192 14.8 us (4.6 TB/s). Every 16 columns more cost 1.5 to 3 us, their codes being read by all 256 workgroups. Two slots
+ * Measured, three sets of operands in turn: 14336 x 1 x 4096 10.5 us (5.6 TB/s), 8192 x 16 x 8192 11.8 us (5.7 TB/s), 8192 x
+ * 48 x 8192 14.5 us (4.7 TB/s). Every 16 columns more cost 1.5 to 3 us, their codes being read by all 256 workgroups. Two slots
  * per wave, the next but one slab under way, change nothing at these sizes. On 128 x 128 tiles 16, 22 and 22 us. */
 #pragma once
 #include "och_gemm_f8_tile.h"
@@ -172,18 +172,19 @@ template <bool E5A, bool E5B, bool WIDE, int TM, int TN> static int gemm_f8_few_
    OCH_CHECK_LAUNCH();
    return 0;
 }
-template <bool E5A, bool E5B, bool WIDE> static int gemm_f8_few_columns(const F8GemmParams &p, hipStream_t stream)
-{
-   if (p.N <= 16) return gemm_f8_few_launch<E5A, E5B, WIDE, 1, 1>(p, stream);
-   /* single tiles of rows where pairs would leave compute units idle: 4096 x 32 x 14336 12.9 us against 16.2 */
-   const bool single = p.M <= 16u * (uint32_t)gemm_compute_units();
-   if (p.N <= 32) return single ? gemm_f8_few_launch<E5A, E5B, WIDE, 1, 2>(p, stream) : gemm_f8_few_launch<E5A, E5B, WIDE, 2, 2>(p, stream);
-   if (p.N <= 48) return single ? gemm_f8_few_launch<E5A, E5B, WIDE, 1, 3>(p, stream) : gemm_f8_few_launch<E5A, E5B, WIDE, 2, 3>(p, stream);
-   return single ? gemm_f8_few_launch<E5A, E5B, WIDE, 1, 4>(p, stream) : gemm_f8_few_launch<E5A, E5B, WIDE, 2, 4>(p, stream);
-}
+/* Up to 32 columns the bfloat16 instructions take 1 % more time at most (8192 x 16 x 8192 11.76 us and 11.71, 8192 x 32 x 8192
+   13.0 and 12.8, 14336 x 1 x 4096 10.5 and 10.4), so 16-bit results have float sums as well. With more columns they would take 3 to
+   20 % (8192 x 48 x 8192 15.4 us and 14.5, 14336 x 64 x 4096 with a scale per row of A 22.6 and 18.8). */
 template <bool E5A, bool E5B> static int gemm_f8_few(const F8GemmParams &p, hipStream_t stream)
 {
-   return p.dtypeC == OCH_FLOAT ? gemm_f8_few_columns<E5A, E5B, true>(p, stream) : gemm_f8_few_columns<E5A, E5B, false>(p, stream);
+   if (p.N <= 16) return gemm_f8_few_launch<E5A, E5B, true, 1, 1>(p, stream);
+   /* single tiles of rows where pairs would leave compute units idle: 4096 x 32 x 14336 12.9 us against 16.2 */
+   const bool single = p.M <= 16u * (uint32_t)gemm_compute_units(), wide = p.dtypeC == OCH_FLOAT;
+   if (p.N <= 32) return single ? gemm_f8_few_launch<E5A, E5B, true, 1, 2>(p, stream) : gemm_f8_few_launch<E5A, E5B, true, 2, 2>(p, stream);
+#define OCH_GO(TN) (single ? (wide ? gemm_f8_few_launch<E5A, E5B, true, 1, TN>(p, stream) : gemm_f8_few_launch<E5A, E5B, false, 1, TN>(p, stream)) \
+                           : (wide ? gemm_f8_few_launch<E5A, E5B, true, 2, TN>(p, stream) : gemm_f8_few_launch<E5A, E5B, false, 2, TN>(p, stream)))
+   return p.N <= 48 ? OCH_GO(3) : OCH_GO(4);
+#undef OCH_GO
 }
 
 } /* namespace och */
