@@ -469,9 +469,10 @@ int och_rms_norm_grad(int dtype, size_t n, size_t rows, const void *dY, ptrdiff_
 /* x features-out and X features-in x tokens: the forward pass is 'T', 'N'; the input's gradient 'N', 'N' with A = W (its  */
 /* 128 x 128 scales serve both); the weights' gradient 'N', 'T' with A = X and B = dY quantized along the tokens.          */
 /* A float result has sums as good as float additions make them, and so has a half or bfloat16 result of up to 32 columns  */
-/* where the order is 'T', 'N' and both operands' starts and leading dimensions are multiples of 16. For the other half    */
-/* and bfloat16 results the 8-bit matrix instruction adds eight products at a time and cuts off what lies below 2^-13 of   */
-/* the largest of them: 4e-5 to 1e-4 of the result's norm, less than the rounding to half.                                 */
+/* where the order is 'T', 'N', both operands' starts and leading dimensions are multiples of 16 and the leading           */
+/* dimensions lie below 2^25, those of the scales below 2^24. For the other half and bfloat16 results the 8-bit matrix     */
+/* instruction adds eight products at a time and cuts off what lies below 2^-13 of the largest of them: 4e-5 to 1e-4 of    */
+/* the result's norm, less than the rounding to half.                                                                      */
 /* The two scales of a block are multiplied with each other first, in float, and their product with the block's sum: it    */
 /* has to be finite, or every result that the block takes part in is infinite or NaN, and at 2^-126 or more for the block  */
 /* to count in full (from 2^-149 down it counts as nothing). Two scales between 2^-63 and 2^63, those of blocks whose      */

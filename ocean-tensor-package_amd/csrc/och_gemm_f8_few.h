@@ -172,7 +172,7 @@ template <bool E5A, bool E5B, bool WIDE, int TM, int TN> static int gemm_f8_few_
    OCH_CHECK_LAUNCH();
    return 0;
 }
-/* Up to 32 columns the bfloat16 instructions take 1 % more time at most (8192 x 16 x 8192 11.76 us and 11.71, 8192 x 32 x 8192
+/* Up to 32 columns the bfloat16 instructions take 0.5 to 1.5 % more time (8192 x 16 x 8192 11.76 us and 11.71, 8192 x 32 x 8192
    13.0 and 12.8, 14336 x 1 x 4096 10.5 and 10.4), so 16-bit results have float sums as well. With more columns they would take 3 to
    20 % (8192 x 48 x 8192 15.4 us and 14.5, 14336 x 64 x 4096 with a scale per row of A 22.6 and 18.8). */
 template <bool E5A, bool E5B> static int gemm_f8_few(const F8GemmParams &p, hipStream_t stream)
